@@ -64,7 +64,8 @@ def draw(rng):
     N = _spread(rng, 16, 4096, rng.choice([1, 8, 64]))
     M = _spread(rng, 1, max(1, min(50432, 80_000_000_000 // (2 * N * K), 35_000_000 // max(N, K))))
     if op == "product":
-        return {"op": op, "M": M, "N": N, "K": K, "a": rng.choice(["mxfp4", "e4m3"]), "out": rng.choice(["bf16", "f32"]),
+        a = rng.choice(["mxfp4", "e4m3"])
+        return {"op": op, "M": M, "N": N, "K": K, "a": a, "out": rng.choice(["bf16", "f32"]) if a == "mxfp4" else "bf16",
                 "bias": rng.random() < 0.7, "res": rng.random() < 0.4}
     return {"op": op, "rows": max(1, min(M, 12608)), "C": K, "N": N, "dtype": dtype}
 
@@ -218,7 +219,7 @@ def _run_plain(s):
     z = (q.float() @ _unpack(*s["W"]).t()) * scale[:, None] + s["bias"]
     dy = _on_grid(s["d"].float()) @ _unpack(*s["WT"]).t()
     dx, dw = _plain_norm_bwd(h.to(t), rstd, dy, s["w"], s["dres"])
-    return {"z": z.to(t), "h": h.to(t), "dx": dx, "dw": dw}
+    return {"z": z.to(torch.bfloat16), "h": h.to(t), "dx": dx, "dw": dw}
 
 
 def _run_own(s):
@@ -243,10 +244,9 @@ def _run_own(s):
         return ops.dequant_mxfp4(*ops.quant_mxfp4(s["x"], transpose=s["transpose"]))
     if op == "product":
         return ops.gemm_mxfp4(s["A"], s["B"], bias=s["bias"], res=s["r"], out_dtype=TYPES[s["out"]])
-    t = s["x"].dtype
     rstd = torch.empty(s["x"].shape[0], dtype=torch.float32, device=s["x"].device)
     n = ops.rmsnorm(s["x"], s["w"], res=s["r"], fmt="e4m3", rstd=rstd, eps=EPS)
-    z = ops.gemm_mxfp4((n["q"], n["scale"]), s["W"], bias=s["bias"], out_dtype=t)
+    z = ops.gemm_mxfp4((n["q"], n["scale"]), s["W"], bias=s["bias"])
     dy = ops.gemm_mxfp4(ops.quant_mxfp4(s["d"]), s["WT"], out_dtype=torch.float32)
     dx, dw = ops.rmsnorm_bwd(n["h"], rstd, dy, s["w"], dres=s["dres"])
     return {"z": z, "h": n["h"], "dx": dx, "dw": dw}
@@ -279,7 +279,7 @@ def work(case):
         a = _four(M, K) if case["a"] == "mxfp4" else M * K + 4 * M
         return {"bytes": a + _four(N, K) + M * N * _size(case["out"]) * (2 if case["res"] else 1) + (4 * N if case["bias"] else 0), "flops": 2 * M * N * K}
     rows, C, N, e = case["rows"], case["C"], case["N"], _size(case["dtype"])
-    return {"bytes": rows * C * e * 5 + rows * N * e * 2 + _four(N, C) + _four(C, N) + 8 * C + 4 * N, "flops": 4 * rows * N * C}
+    return {"bytes": rows * C * e * 5 + rows * N * (e + 2) + _four(N, C) + _four(C, N) + 8 * C + 4 * N, "flops": 4 * rows * N * C}
 
 
 # ---- the definition in 64 bits ------------------------------------------------------------------------------------------------------------------------
