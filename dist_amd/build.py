@@ -12,7 +12,8 @@ SOURCES = ["gemm_nt.hip", "gemm_fast.hip", "gemm_small.hip", "gemm_tn.hip", "gem
 MEASURE_SOURCES = [os.path.join("measure", "gemm_pp.hip"), os.path.join("measure", "integ4.hip")]
 HEADERS = ["common.h", "kernels.h", "engine_internal.h", "integ_common.h", os.path.join("..", "..", "include", "dist_amd.h"),
            os.path.join("measure", "gemm_fast8q.inl"), os.path.join("measure", "gemm_fast8q_launch.inl")]
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wno-unused-result"]
+# (-packed-fp32-ops: -O3 forms packed fp32 instructions from plain float code, and some of their forms have given wrong results now and then)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _stale(target, deps):
@@ -38,7 +39,7 @@ def build_library(force=False, verbose=True, measure=False):
     lib = MEASURE_LIB if measure else LIB
     osuf = ".m.o" if measure else ".o"
     key_file = os.path.join(CSRC, ".defs.measure" if measure else ".defs")
-    key = " ".join(defs)
+    key = " ".join(FLAGS + defs)
     if (open(key_file).read() if os.path.exists(key_file) else "") != key:
         force = True
     hdrs = [os.path.join(CSRC, h) for h in HEADERS]
