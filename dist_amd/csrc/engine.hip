@@ -391,6 +391,7 @@ extern "C" int dist_abi_sizeof(const char* n) {
 #define DIST_SZ(T) if (!strcmp(n, #T)) return (int)sizeof(T)
     DIST_SZ(dist_gemm_args); DIST_SZ(dist_gemm_tn_args); DIST_SZ(dist_ln_args); DIST_SZ(dist_ln_bwd_args);
     DIST_SZ(dist_adamw_seg); DIST_SZ(dist_config); DIST_SZ(dist_rowmap); DIST_SZ(dist_outmap); DIST_SZ(dist_tnet_args); DIST_SZ(dist_tnet_bwd_args); DIST_SZ(dist_integ_args); DIST_SZ(dist_integ_pack_args); DIST_SZ(dist_integ_unfold_args); DIST_SZ(dist_integ_bwd_args);
+    DIST_SZ(dist_rms_args); DIST_SZ(dist_rms_bwd_args); DIST_SZ(dist_gemm_mx_args);
 #undef DIST_SZ
     return -1;
 }

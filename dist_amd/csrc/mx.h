@@ -1,0 +1,71 @@
+// Microscaled 4-bit floating point (MXFP4): the element grid, the shared scale and the storage layout, used by mxfp4.hip, rmsnorm.hip and gemm_mx.hip.
+//
+// Elements are e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), 32 along the quantised axis share one power of two 2^(byte - 127):
+//   byte = max(floor(log2(max |x|)) + 127 - 2, 0);  code = e2m1(x / 2^(byte - 127)), nearest, ties to the even code, magnitudes above 6 -> 6.
+// An infinity or a NaN in a block makes its byte 255 (the format's NaN): the block reads back, and multiplies, as NaN.
+// Codes: row-major bytes, element 2i in the low half of byte i, rows padded with zeros to a whole block of 32.
+// Scales: [chunk of 256 elements][row][8 bytes], byte 2 g + s of a chunk = block 4 s + g.  v_mfma_scale_f32_16x16x128_f8f6f4 takes the scale of lane group g (block
+// g of its 128 elements) from a byte of that lane's register, the byte's number being part of the instruction: the two bytes of a lane group are its operands of
+// two consecutive K steps, one 16-bit load each.  A chunk's scales of neighbouring rows are contiguous, so a tile of rows stages them as one run.
+#pragma once
+#include "common.h"
+
+namespace mx {
+
+constexpr int BLOCK = 32, CHUNK = 256;
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+DEV unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }       // ordered like |x|, with infinity and then NaN on top: maxima keep them
+DEV int scale_byte(unsigned amax_bits) {
+    const int e = (int)(amax_bits >> 23);
+    return e == 255 ? 255 : max(e - 2, 0);
+}
+DEV float scale_value(int byte) { return __uint_as_float(byte == 0 ? 0x00400000u : (unsigned)byte << 23); }   // byte 255: NaN or infinity bits, never used as a divisor
+// position of block b (of the whole row) inside the scales of `rows` rows
+DEV long scale_at(long row, long rows, int b) { return ((long)(b >> 3) * rows + row) * 8 + 2 * (b & 3) + ((b >> 2) & 1); }
+
+// eight values -> eight codes, first value in the low half of the first byte.  v_cvt_scalef32_pk_fp4_f32 divides by its scale operand and rounds to nearest even
+// with saturation; checked against the definition for every bf16 value at twelve scales, the subnormal one among them.
+DEV unsigned pack8(const float v[8], int byte) {
+    if (byte == 255) return 0u;
+    const float s = scale_value(byte);
+    unsigned w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], s, 3);
+    return w;
+}
+DEV void unpack8(unsigned w, int byte, float v[8]) {
+    const float s = scale_value(byte);
+    const f32x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+    const f32x2_t c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
+    v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1]; v[4] = c[0]; v[5] = c[1]; v[6] = d[0]; v[7] = d[1];
+    if (byte == 255) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(0x7fc00000u);
+    }
+}
+
+// V consecutive elements (V = 8: 16-byte aligned) <-> fp32
+template <int V> DEV void load_v(const float* p, float o[V]) {
+    if constexpr (V == 8) { Frag<float> f; frag_load(f, p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = f.v[e]; }
+    else o[0] = *p;
+}
+template <int V> DEV void load_v(const bf16_t* p, float o[V]) {
+    if constexpr (V == 8) { Frag<bf16_t> f; frag_load(f, p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = (float)f.v[e]; }
+    else o[0] = (float)*p;
+}
+template <int V, typename T> DEV void store_v(T* p, const float o[V]) {
+    if constexpr (V == 8) { Frag<T> f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) frag_set(f, e, o[e]);
+        frag_store(f, p); }
+    else *p = from_f<T>(o[0]);
+}
+
+}  // namespace mx

@@ -1,0 +1,411 @@
+// Root-mean-square norm with the residual's addition (dist_op_rmsnorm) and its backward (dist_op_rmsnorm_bwd).
+//   h = x + res;  rstd = 1 / sqrt(mean_c h^2 + eps);  y = h rstd w
+//   g = dy w, n = h rstd:  dh = rstd (g - n mean_c(g n)) + dres;  dw = sum_rows dy n
+// HBM-bound: a row is read once and stays in the registers of its lanes between the statistics and the output, which is y in the input's type, y in e4m3 with one
+// scale per row, or y in MXFP4 - the operands of dist_op_gemm_nt (DIST_EPI_FP8) and dist_op_gemm_mxfp4 - so that no separate quantisation pass reads y again.
+// Everything between the loads and the one rounding of an output is fp32: y is formed from the unrounded x + res, not from the stored h.
+#include "mx.h"
+
+namespace {
+
+constexpr int NT = 256;
+
+// sum / maximum over the LPR lanes that own a row; every lane gets the result.  LPR = 256: the whole block, `red` = 4 words of LDS, fixed order
+template <int LPR> DEV float row_sum(float v, float* red) {
+    if constexpr (LPR <= 64) return wave_sum(v, LPR);
+    v = wave_sum(v, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+template <int LPR> DEV float row_max(float v, float* red) {
+    if constexpr (LPR <= 64) return wave_max(v, LPR);
+    v = wave_max(v, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// e4m3 factor and scale of a row whose largest |y| is a: those of dist_op_quant_rows_fp8 down to 2^-100; below that a counts as 2^-100 (448 / a would overflow)
+DEV float e4m3_factor(float a, float& scale) {
+    const float b = fmaxf(a, 7.8886090522101181e-31f);
+    scale = a > 0.f ? b / 448.f : 1.f;
+    return a > 0.f ? 448.f / b : 1.f;
+}
+
+// one group of V values of a row -> the output of format FMT; `lanes` of a block of 32 elements are 32 / V neighbours and all of them call
+template <typename T, int V, int FMT>
+DEV void put(const dist_rms_args& p, const float y[V], float inv, long row, long c, int Kp) {
+    if constexpr (FMT == DIST_RMS_SAME) {
+        if (c < p.C) mx::store_v<V>(static_cast<T*>(p.y) + row * p.ldy + c, y);
+    } else if constexpr (FMT == DIST_RMS_E4M3) {
+        unsigned char* q = static_cast<unsigned char*>(p.y) + row * p.ldy + c;
+        if constexpr (V == 8) {
+            if (c < p.C) {
+                int lo = 0, hi = 0;
+                lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * inv, y[1] * inv, lo, false);
+                lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * inv, y[3] * inv, lo, true);
+                hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4] * inv, y[5] * inv, hi, false);
+                hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6] * inv, y[7] * inv, hi, true);
+                *reinterpret_cast<int2*>(q) = make_int2(lo, hi);
+            }
+        } else if (c < p.C) *q = (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(y[0] * inv, 0.f, 0, false) & 0xff);
+    } else {
+        unsigned a = 0;
+#pragma unroll
+        for (int e = 0; e < V; ++e) a = max(a, mx::abs_bits(y[e]));
+#pragma unroll
+        for (int o = 1; o < 32 / V; o *= 2) a = max(a, (unsigned)__shfl_xor((int)a, o, 64));
+        const int byte = mx::scale_byte(a);
+        unsigned char* q = static_cast<unsigned char*>(p.y) + row * (Kp / 2) + c / 2;
+        if constexpr (V == 8) {
+            if (c < Kp) *reinterpret_cast<unsigned*>(q) = mx::pack8(y, byte);
+        } else {
+            const float other = __shfl_xor(y[0], 1, 64);
+            if (c < Kp && (c & 1) == 0)
+                *q = byte == 255 ? 0 : (unsigned char)(__builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], other, mx::scale_value(byte), 0) & 0xff);
+        }
+        if (c % 32 == 0 && c < (long)(Kp + 255) / 256 * 256) static_cast<unsigned char*>(p.scale)[mx::scale_at(row, p.rows, (int)(c / 32))] = (unsigned char)(c < Kp ? byte : 0);
+    }
+}
+
+// LPR lanes own a row and hold IT groups of V elements each (V = 8: aligned rows of whole groups; V = 1: any width and alignment)
+template <typename T, int V, int LPR, int IT, int FMT>
+__global__ __launch_bounds__(NT) void rms_fwd_kernel(const dist_rms_args p) {
+    __shared__ float red[4];
+    const int lr = threadIdx.x % LPR;
+    const long row = (long)blockIdx.x * (NT / LPR) + threadIdx.x / LPR;
+    if (row >= p.rows) return;
+    const int C = p.C, Kp = (C + 31) / 32 * 32;
+    const T* X = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* R = p.res ? static_cast<const T*>(p.res) + row * p.ldres : nullptr;
+    float x[IT][V];
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+        const int c = (lr + it * LPR) * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[it][e] = 0.f;
+        if (c < C) mx::load_v<V>(X + c, x[it]);
+    }
+    if (R) {
+#pragma unroll
+        for (int it = 0; it < IT; ++it) {
+            const int c = (lr + it * LPR) * V;
+            if (c < C) {
+                float r[V];
+                mx::load_v<V>(R + c, r);
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[it][e] += r[e];
+            }
+        }
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int it = 0; it < IT; ++it)
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += x[it][e] * x[it][e];
+    const float rstd = 1.f / sqrtf(row_sum<LPR>(s, red) / (float)C + p.eps);
+    if (p.rstd && lr == 0) p.rstd[row] = rstd;
+    if (p.h) {
+        T* H = static_cast<T*>(p.h) + row * p.ldh;
+#pragma unroll
+        for (int it = 0; it < IT; ++it) {
+            const int c = (lr + it * LPR) * V;
+            if (c < C) mx::store_v<V>(H + c, x[it]);
+        }
+    }
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+        const int c = (lr + it * LPR) * V;
+        if (c < C) {
+            float w[V];
+            mx::load_v<V>(p.w + c, w);
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[it][e] = x[it][e] * rstd * w[e];
+        }
+    }
+    float inv = 1.f;
+    if constexpr (FMT == DIST_RMS_E4M3) {
+        float a = 0.f, scale;
+#pragma unroll
+        for (int it = 0; it < IT; ++it)
+#pragma unroll
+            for (int e = 0; e < V; ++e) a = fmaxf(a, fabsf(x[it][e]));
+        inv = e4m3_factor(row_max<LPR>(a, red), scale);
+        if (lr == 0) static_cast<float*>(p.scale)[row] = scale;
+    }
+#pragma unroll
+    for (int it = 0; it < IT; ++it) put<T, V, FMT>(p, x[it], inv, row, (long)(lr + it * LPR) * V, Kp);
+}
+
+// rows too long for the registers: the block walks its row again for every step (the second and third walk find it in the L2).  h is stored last, so it may be x or res.
+template <typename T, int FMT>
+__global__ __launch_bounds__(NT) void rms_fwd_long_kernel(const dist_rms_args p) {
+    __shared__ float red[4];
+    const long row = blockIdx.x;
+    const int C = p.C, Kp = (C + 31) / 32 * 32, tid = threadIdx.x;
+    const T* X = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* R = p.res ? static_cast<const T*>(p.res) + row * p.ldres : nullptr;
+    T* H = p.h ? static_cast<T*>(p.h) + row * p.ldh : nullptr;
+    float s = 0.f;
+    for (long c = tid; c < C; c += NT) { const float h = to_f(X[c]) + (R ? to_f(R[c]) : 0.f); s += h * h; }
+    const float rstd = 1.f / sqrtf(row_sum<NT>(s, red) / (float)C + p.eps);
+    if (p.rstd && tid == 0) p.rstd[row] = rstd;
+    float inv = 1.f;
+    if constexpr (FMT == DIST_RMS_E4M3) {
+        float a = 0.f, scale;
+        for (long c = tid; c < C; c += NT) a = fmaxf(a, fabsf((to_f(X[c]) + (R ? to_f(R[c]) : 0.f)) * rstd * p.w[c]));
+        inv = e4m3_factor(row_max<NT>(a, red), scale);
+        if (tid == 0) static_cast<float*>(p.scale)[row] = scale;
+    }
+    for (long c = tid; c < ((long)C + NT - 1) / NT * NT; c += NT) {          // (whole chunks: every lane of a block of 32 takes part)
+        float y = 0.f;
+        if (c < C) {
+            const float h = to_f(X[c]) + (R ? to_f(R[c]) : 0.f);
+            y = h * rstd * p.w[c];
+            if (H) H[c] = from_f<T>(h);
+        }
+        put<T, 1, FMT>(p, &y, inv, row, c, Kp);
+    }
+}
+
+// Backward.  A block keeps the sums of dw over its rows in registers and leaves one partial row; rms_dw_kernel adds the partial rows in a fixed order (no atomics:
+// the same bits every time).
+template <typename T, typename TD, int V, int LPR, int IT>
+__global__ __launch_bounds__(NT) void rms_bwd_kernel(const dist_rms_bwd_args p) {
+    __shared__ float red[4];
+    __shared__ float cols[LPR < NT ? LPR * IT * V : 1];
+    const int lr = threadIdx.x % LPR, slot = threadIdx.x / LPR, C = p.C;
+    constexpr int RPB = NT / LPR;
+    float w[IT][V], aw[IT][V];
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+        const int c = (lr + it * LPR) * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[it][e] = aw[it][e] = 0.f;
+        if (c < C) mx::load_v<V>(p.w + c, w[it]);
+    }
+    for (long row = (long)blockIdx.x * RPB + slot; row < p.rows; row += (long)gridDim.x * RPB) {
+        const T* H = static_cast<const T*>(p.h) + row * p.ldh;
+        const TD* D = static_cast<const TD*>(p.dy) + row * p.lddy;
+        const float rstd = p.rstd[row];
+        float n[IT][V], g[IT][V];
+#pragma unroll
+        for (int it = 0; it < IT; ++it) {
+            const int c = (lr + it * LPR) * V;
+#pragma unroll
+            for (int e = 0; e < V; ++e) n[it][e] = g[it][e] = 0.f;
+            if (c < C) { mx::load_v<V>(H + c, n[it]); mx::load_v<V>(D + c, g[it]); }
+        }
+        float s = 0.f;
+#pragma unroll
+        for (int it = 0; it < IT; ++it)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                n[it][e] *= rstd;
+                aw[it][e] += g[it][e] * n[it][e];
+                g[it][e] *= w[it][e];
+                s += g[it][e] * n[it][e];
+            }
+        const float m = row_sum<LPR>(s, red) / (float)C;
+        if (p.dh) {
+            T* O = static_cast<T*>(p.dh) + row * p.lddh;
+            const T* A = p.dres ? static_cast<const T*>(p.dres) + row * p.lddres : nullptr;
+#pragma unroll
+            for (int it = 0; it < IT; ++it) {
+                const int c = (lr + it * LPR) * V;
+                if (c < C) {
+                    float o[V], a[V];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) a[e] = 0.f;
+                    if (A) mx::load_v<V>(A + c, a);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) o[e] = rstd * (g[it][e] - n[it][e] * m) + a[e];
+                    mx::store_v<V>(O + c, o);
+                }
+            }
+        }
+    }
+    float* part = p.scratch + (long)blockIdx.x * C;
+    if constexpr (LPR == NT) {
+#pragma unroll
+        for (int it = 0; it < IT; ++it) {
+            const int c = (lr + it * LPR) * V;
+            if (c < C)
+#pragma unroll
+                for (int e = 0; e < V; ++e) part[c + e] = aw[it][e];
+        }
+    } else {
+        for (int k = 0; k < RPB; ++k) {                                       // the block's row slots, one after the other
+            if (slot == k) {
+#pragma unroll
+                for (int it = 0; it < IT; ++it)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        float& o = cols[(lr + it * LPR) * V + e];
+                        o = k == 0 ? aw[it][e] : o + aw[it][e];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < C; c += NT) part[c] = cols[c];
+    }
+}
+
+// long rows: dh by a block per row; dw by columns, one partial row per slice of rows
+template <typename T, typename TD>
+__global__ __launch_bounds__(NT) void rms_bwd_long_kernel(const dist_rms_bwd_args p) {
+    __shared__ float red[4];
+    const long row = blockIdx.x;
+    const int C = p.C;
+    const T* H = static_cast<const T*>(p.h) + row * p.ldh;
+    const TD* D = static_cast<const TD*>(p.dy) + row * p.lddy;
+    const T* A = p.dres ? static_cast<const T*>(p.dres) + row * p.lddres : nullptr;
+    T* O = static_cast<T*>(p.dh) + row * p.lddh;
+    const float rstd = p.rstd[row];
+    float s = 0.f;
+    for (long c = threadIdx.x; c < C; c += NT) s += to_f(D[c]) * p.w[c] * (to_f(H[c]) * rstd);
+    const float m = row_sum<NT>(s, red) / (float)C;
+    for (long c = threadIdx.x; c < C; c += NT) O[c] = from_f<T>(rstd * (to_f(D[c]) * p.w[c] - to_f(H[c]) * rstd * m) + (A ? to_f(A[c]) : 0.f));
+}
+template <typename T, typename TD>
+__global__ __launch_bounds__(NT) void rms_dw_cols_kernel(const dist_rms_bwd_args p, const int slices, const int ctiles) {
+    const int slice = blockIdx.x / ctiles;
+    const long c = (long)(blockIdx.x % ctiles) * NT + threadIdx.x;
+    if (c >= p.C) return;
+    float s = 0.f;
+    for (long row = slice; row < p.rows; row += slices)
+        s += to_f(static_cast<const TD*>(p.dy)[row * p.lddy + c]) * (to_f(static_cast<const T*>(p.h)[row * p.ldh + c]) * p.rstd[row]);
+    p.scratch[(long)slice * p.C + c] = s;
+}
+
+// dw[c] (+)= sum of the partial rows: 16 groups of 64 threads take every 16th row each, then the groups in order
+__global__ __launch_bounds__(1024) void rms_dw_kernel(const float* __restrict__ part, const int G, const int C, float* __restrict__ dw, const int accumulate) {
+    __shared__ float red[16][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6;
+    float s = 0.f;
+    if (c < C) {
+#pragma unroll 8
+        for (int k = g; k < G; k += 16) s += part[(long)k * C + c];
+    }
+    red[g][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (g == 0 && c < C) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k) s += red[k][threadIdx.x];
+        dw[c] = accumulate ? dw[c] + s : s;
+    }
+}
+
+constexpr int VEC_MAX = 16384, ONE_MAX = 4096;                 // widths the register-resident kernels take
+constexpr int BWD_VEC_MAX = 8192, BWD_ONE_MAX = 4096;
+
+// lanes per row of the backward kernel for this width and vector length (0: a long row)
+inline int bwd_lanes(int C, bool vec) {
+    if (vec) return C <= 384 ? 16 : C <= 768 ? 32 : C <= 2048 ? 64 : C <= BWD_VEC_MAX ? 256 : 0;
+    return C <= 1024 ? 64 : C <= BWD_ONE_MAX ? 256 : 0;
+}
+inline int64_t bwd_partials(int64_t rows, int C, bool vec) {
+    const int lanes = bwd_lanes(C, vec);
+    if (!lanes) return rows < 64 ? (rows < 1 ? 1 : rows) : 64;
+    const int64_t need = (rows + NT / lanes - 1) / (NT / lanes);
+    return need < 1 ? 1 : need > 1024 ? 1024 : need;
+}
+inline bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+template <typename T, int FMT> int fwd(const dist_rms_args& p, hipStream_t s) {
+    bool vec = p.C % 8 == 0 && p.ldx % 8 == 0 && aligned16(p.x) && aligned16(p.w) && (!p.res || (p.ldres % 8 == 0 && aligned16(p.res))) &&
+               (!p.h || (p.ldh % 8 == 0 && aligned16(p.h))) && aligned16(p.y);
+    if (FMT != DIST_RMS_MXFP4) vec = vec && p.ldy % 8 == 0;
+    const int64_t Cr = FMT == DIST_RMS_MXFP4 ? ((int64_t)p.C + 255) / 256 * 256 : p.C;       // (the scale bytes of a whole chunk are written)
+    const int64_t rows = p.rows;
+#define DIST_RMS(V, LPR, IT) do { const int64_t b = (rows + NT / LPR - 1) / (NT / LPR); if (b > 0x7fffffff) return DIST_ERR_ARG; \
+        hipLaunchKernelGGL((rms_fwd_kernel<T, V, LPR, IT, FMT>), dim3((unsigned)b), dim3(NT), 0, s, p); } while (0)
+    if (vec && Cr <= VEC_MAX) {
+        if (Cr <= 384) DIST_RMS(8, 16, 3);
+        else if (Cr <= 768) DIST_RMS(8, 32, 3);
+        else if (Cr <= 1024) DIST_RMS(8, 64, 2);
+        else if (Cr <= 2048) DIST_RMS(8, 64, 4);
+        else if (Cr <= 4096) DIST_RMS(8, 256, 2);
+        else if (Cr <= 8192) DIST_RMS(8, 256, 4);
+        else DIST_RMS(8, 256, 8);
+    } else if (Cr <= ONE_MAX) {
+        if (Cr <= 1024) DIST_RMS(1, 64, 16);
+        else if (Cr <= 2048) DIST_RMS(1, 256, 8);
+        else DIST_RMS(1, 256, 16);
+    } else {
+        if (rows > 0x7fffffff) return DIST_ERR_ARG;
+        hipLaunchKernelGGL((rms_fwd_long_kernel<T, FMT>), dim3((unsigned)rows), dim3(NT), 0, s, p);
+    }
+#undef DIST_RMS
+    HIP_CHECK_RET(hipGetLastError());
+    return DIST_OK;
+}
+
+template <typename T, typename TD> int bwd(const dist_rms_bwd_args& p, bool vec, hipStream_t s) {
+    const int G = (int)bwd_partials(p.rows, p.C, vec);
+    const int lanes = bwd_lanes(p.C, vec);
+#define DIST_RMS(V, LPR, IT) hipLaunchKernelGGL((rms_bwd_kernel<T, TD, V, LPR, IT>), dim3((unsigned)G), dim3(NT), 0, s, p)
+    if (!lanes) {
+        if (p.rows > 0x7fffffff) return DIST_ERR_ARG;
+        const int ctiles = (p.C + NT - 1) / NT;
+        if (p.dh && p.rows) hipLaunchKernelGGL((rms_bwd_long_kernel<T, TD>), dim3((unsigned)p.rows), dim3(NT), 0, s, p);
+        hipLaunchKernelGGL((rms_dw_cols_kernel<T, TD>), dim3((unsigned)(G * ctiles)), dim3(NT), 0, s, p, G, ctiles);
+    } else if (vec) {
+        if (lanes == 16) DIST_RMS(8, 16, 3);
+        else if (lanes == 32) DIST_RMS(8, 32, 3);
+        else if (lanes == 64) { if (p.C <= 1024) DIST_RMS(8, 64, 2); else DIST_RMS(8, 64, 4); }
+        else { if (p.C <= 4096) DIST_RMS(8, 256, 2); else DIST_RMS(8, 256, 4); }
+    } else {
+        if (lanes == 64) DIST_RMS(1, 64, 16);
+        else DIST_RMS(1, 256, 16);
+    }
+#undef DIST_RMS
+    HIP_CHECK_RET(hipGetLastError());
+    hipLaunchKernelGGL(rms_dw_kernel, dim3((unsigned)((p.C + 63) / 64)), dim3(1024), 0, s, p.scratch, G, p.C, p.dw, p.accumulate);
+    HIP_CHECK_RET(hipGetLastError());
+    return DIST_OK;
+}
+
+}  // namespace
+
+extern "C" int dist_op_rmsnorm(const dist_rms_args* a, void* stream) {
+    if (!a) return DIST_ERR_ARG;
+    const dist_rms_args p = *a;
+    if (p.dtype != DIST_BF16 && p.dtype != DIST_F32) return DIST_ERR_ARG;
+    if (p.fmt != DIST_RMS_SAME && p.fmt != DIST_RMS_E4M3 && p.fmt != DIST_RMS_MXFP4) return DIST_ERR_ARG;
+    if (p.rows < 0 || p.C <= 0 || p.C > (1 << 30) || !(p.eps >= 0.f)) return DIST_ERR_ARG;
+    if (p.rows == 0) return DIST_OK;
+    const uintptr_t es = p.dtype == DIST_BF16 ? 2 : 4;
+    if (!p.x || !p.w || !p.y || (p.fmt != DIST_RMS_SAME && !p.scale) || p.ldx < p.C || (p.res && p.ldres < p.C) || (p.h && p.ldh < p.C)) return DIST_ERR_ARG;
+    if (p.fmt != DIST_RMS_MXFP4 && p.ldy < p.C) return DIST_ERR_ARG;
+    if ((uintptr_t)p.x % es || (uintptr_t)p.res % es || (uintptr_t)p.h % es || (p.fmt == DIST_RMS_SAME && (uintptr_t)p.y % es) || (p.fmt == DIST_RMS_MXFP4 && !aligned16(p.y))) return DIST_ERR_ARG;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (p.dtype == DIST_BF16)
+        return p.fmt == DIST_RMS_SAME ? fwd<bf16_t, DIST_RMS_SAME>(p, s) : p.fmt == DIST_RMS_E4M3 ? fwd<bf16_t, DIST_RMS_E4M3>(p, s) : fwd<bf16_t, DIST_RMS_MXFP4>(p, s);
+    return p.fmt == DIST_RMS_SAME ? fwd<float, DIST_RMS_SAME>(p, s) : p.fmt == DIST_RMS_E4M3 ? fwd<float, DIST_RMS_E4M3>(p, s) : fwd<float, DIST_RMS_MXFP4>(p, s);
+}
+
+extern "C" int64_t dist_op_rmsnorm_bwd_scratch(int64_t rows, int C) {
+    if (rows < 0 || C <= 0) return -1;
+    const int64_t a = bwd_partials(rows, C, true), b = bwd_partials(rows, C, false);
+    return (a > b ? a : b) * C;
+}
+
+extern "C" int dist_op_rmsnorm_bwd(const dist_rms_bwd_args* a, void* stream) {
+    if (!a) return DIST_ERR_ARG;
+    const dist_rms_bwd_args p = *a;
+    if ((p.dtype != DIST_BF16 && p.dtype != DIST_F32) || (p.dy_dtype != DIST_BF16 && p.dy_dtype != DIST_F32)) return DIST_ERR_ARG;
+    if (p.rows < 0 || p.C <= 0 || p.C > (1 << 30) || !p.w || !p.dw || !p.scratch) return DIST_ERR_ARG;
+    if (p.scratch_elems < dist_op_rmsnorm_bwd_scratch(p.rows, p.C)) return DIST_ERR_WORKSPACE;
+    if (p.rows > 0 && (!p.h || !p.rstd || !p.dy || p.ldh < p.C || p.lddy < p.C || (p.dres && p.lddres < p.C) || (p.dh && p.lddh < p.C))) return DIST_ERR_ARG;
+    const uintptr_t es = p.dtype == DIST_BF16 ? 2 : 4, ed = p.dy_dtype == DIST_BF16 ? 2 : 4;
+    if ((uintptr_t)p.h % es || (uintptr_t)p.dres % es || (uintptr_t)p.dh % es || (uintptr_t)p.dy % ed) return DIST_ERR_ARG;
+    const bool vec = p.C % 8 == 0 && p.ldh % 8 == 0 && p.lddy % 8 == 0 && aligned16(p.h) && aligned16(p.dy) && aligned16(p.w) &&
+                     (!p.dres || (p.lddres % 8 == 0 && aligned16(p.dres))) && (!p.dh || (p.lddh % 8 == 0 && aligned16(p.dh)));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (p.dtype == DIST_BF16) return p.dy_dtype == DIST_BF16 ? bwd<bf16_t, bf16_t>(p, vec, s) : bwd<bf16_t, float>(p, vec, s);
+    return p.dy_dtype == DIST_BF16 ? bwd<float, bf16_t>(p, vec, s) : bwd<float, float>(p, vec, s);
+}

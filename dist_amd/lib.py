@@ -12,6 +12,8 @@ OM_PLAIN, OM_DUP, OM_INSERTCLS, OM_SPLITCOLS, OM_HEADS = range(5)
 QKV_ROWS, QKV_HEADS = 0, 1
 EPI_BIAS, EPI_MULG, EPI_RES, EPI_ACT2, EPI_MULG_POST, EPI_LNFOLD, EPI_ROWSTATS, EPI_FP8 = 1, 2, 4, 8, 16, 32, 64, 128
 EPI_FP8_ASCALAR, EPI_OUT8 = 256, 512
+RMS_SAME, RMS_E4M3, RMS_MXFP4 = range(3)
+MX_A_MXFP4, MX_A_E4M3 = range(2)
 
 
 class RowMap(C.Structure):
@@ -94,6 +96,21 @@ class IntegBwdArgs(C.Structure):
                [(n, C.c_void_p) for n in ("i2t_dXnext", "i2t_B", "i2t_dY", "t2i_B", "t2i_p", "t2i_dp", "t2i_dcls")] + [("dM_cls_only", C.c_int)]
 
 
+class RmsArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "res", "h", "w", "y", "scale", "rstd")] + [(n, C.c_int64) for n in ("rows", "ldx", "ldres", "ldh", "ldy")] + \
+               [(n, C.c_int) for n in ("C", "fmt", "dtype")] + [("eps", C.c_float)]
+
+
+class RmsBwdArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("h", "rstd", "dy", "w", "dres", "dh", "dw", "scratch")] + \
+               [(n, C.c_int64) for n in ("scratch_elems", "rows", "ldh", "lddy", "lddres", "lddh")] + [(n, C.c_int) for n in ("C", "dtype", "dy_dtype", "accumulate")]
+
+
+class GemmMxArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("A", "a_scale", "B", "b_scale", "bias", "res", "C", "scratch")] + \
+               [(n, C.c_int64) for n in ("M", "lda", "ldc", "ldres", "scratch_elems")] + [(n, C.c_int) for n in ("N", "K", "a_fmt", "dtype")]
+
+
 class AdamwSeg(C.Structure):
     _fields_ = [("begin", C.c_int64), ("end", C.c_int64), ("lr", C.c_float), ("weight_decay", C.c_float)]
 
@@ -110,7 +127,8 @@ GRAD_HOOK = C.CFUNCTYPE(None, C.c_void_p, C.c_int64, C.c_int64)
 ABI_VERSION = 9    # include/dist_amd.h DIST_ABI_VERSION: bumped on every struct-layout change
 ABI_MIRRORS = (("dist_gemm_args", GemmArgs), ("dist_gemm_tn_args", GemmTnArgs), ("dist_ln_args", LnArgs), ("dist_ln_bwd_args", LnBwdArgs),
                ("dist_adamw_seg", AdamwSeg), ("dist_config", Config), ("dist_rowmap", RowMap), ("dist_outmap", OutMap), ("dist_tnet_args", TnetArgs), ("dist_tnet_bwd_args", TnetBwdArgs),
-               ("dist_integ_args", IntegArgs), ("dist_integ_pack_args", IntegPackArgs), ("dist_integ_unfold_args", IntegUnfoldArgs), ("dist_integ_bwd_args", IntegBwdArgs))
+               ("dist_integ_args", IntegArgs), ("dist_integ_pack_args", IntegPackArgs), ("dist_integ_unfold_args", IntegUnfoldArgs), ("dist_integ_bwd_args", IntegBwdArgs),
+               ("dist_rms_args", RmsArgs), ("dist_rms_bwd_args", RmsBwdArgs), ("dist_gemm_mx_args", GemmMxArgs))
 
 
 class DistError(RuntimeError):
@@ -239,6 +257,14 @@ def load():
     _sig(lib, "dist_op_fp8_scale_update", argtypes=[C.c_void_p, C.c_void_p, C.c_int, C.c_float, C.c_void_p])
     _sig(lib, "dist_op_amax", argtypes=[C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_void_p])
     _sig(lib, "dist_op_fp8_rowsum", argtypes=[C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p])
+    _sig(lib, "dist_op_rmsnorm", argtypes=[C.POINTER(RmsArgs), C.c_void_p])
+    _sig(lib, "dist_op_rmsnorm_bwd", argtypes=[C.POINTER(RmsBwdArgs), C.c_void_p])
+    _sig(lib, "dist_op_rmsnorm_bwd_scratch", argtypes=[C.c_int64, C.c_int], restype=C.c_int64)
+    _sig(lib, "dist_op_mxfp4_scale_bytes", argtypes=[C.c_int64, C.c_int64], restype=C.c_int64)
+    _sig(lib, "dist_op_quant_mxfp4", argtypes=[C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p])
+    _sig(lib, "dist_op_dequant_mxfp4", argtypes=[C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_void_p])
+    _sig(lib, "dist_op_gemm_mxfp4", argtypes=[C.POINTER(GemmMxArgs), C.c_void_p])
+    _sig(lib, "dist_op_gemm_mxfp4_scratch", argtypes=[C.c_int64, C.c_int, C.c_int, C.c_int], restype=C.c_int64)
     _sig(lib, "dist_op_softmax_rows", argtypes=[C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p])
     _sig(lib, "dist_op_topk_correct", argtypes=[C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_int), C.c_int, C.c_void_p, C.c_void_p])
     _sig(lib, "dist_op_ensemble_update", argtypes=[C.c_void_p] * 6 + [C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p])

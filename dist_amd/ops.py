@@ -547,3 +547,223 @@ def attention_fp8(qkv8, in_scale, frames, Ltok, heads, out8_scale=None, amax=Non
     out8 = torch.empty(frames * Ltok, heads * 64, dtype=torch.uint8, device=qkv8.device)
     L.check(L.load().dist_op_attention_fp8(_p(qkv8), _p(in_scale), None, _p(out8), _p(out8_scale), _p(amax), frames, Ltok, heads, _stream()))
     return out8
+
+
+# ---- a 4-bit frozen linear layer: norm, microscaled 4-bit quantisation, product ---------------------------------------------------------------------------------
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *_):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+RMS_FMTS = {"same": L.RMS_SAME, "e4m3": L.RMS_E4M3, "mxfp4": L.RMS_MXFP4}
+
+
+def _need(ok, what):
+    if not ok:
+        raise L.DistError(what)
+
+
+def _on_device(first, *others):
+    """every tensor on the GPU of `first`; returns the context in which the launch happens (that GPU current, so its current stream is the one used)"""
+    dev = first.device
+    _need(first.is_cuda, "the operands must be GPU tensors")
+    for t in others:
+        _need(t is None or t.device == dev, f"operands on different devices: {dev} and {t.device if t is not None else None}")
+    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _rows(t, rows, cols, what, dtype=None):
+    """a [rows, cols] tensor whose rows are contiguous and do not overlap; returns the row pitch in elements"""
+    _need(t.dim() == 2 and t.shape[0] == rows and t.shape[1] == cols, f"{what}: expected shape {(rows, cols)}, got {tuple(t.shape)}")
+    _need(dtype is None or t.dtype == dtype, f"{what}: expected {dtype}, got {t.dtype}")
+    ld = t.stride(0) if rows > 1 else cols
+    _need((cols == 1 or t.stride(1) == 1) and ld >= cols, f"{what}: rows must be contiguous and must not overlap (strides {t.stride()})")
+    return ld
+
+
+def _vector(t, n, what, dtype=torch.float32):
+    _need(t.dtype == dtype and t.numel() == n and t.is_contiguous(), f"{what}: expected {n} contiguous {dtype} values, got {t.dtype} {tuple(t.shape)}")
+
+
+def _span(t):
+    """first and last byte address of a [rows, cols] tensor"""
+    return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+
+
+def _apart(out, other, what, same_ok=True):
+    """an output may be one of its inputs itself (same address, pitch and type) but must not overlap it otherwise"""
+    if out is None or other is None or out.numel() == 0 or other.numel() == 0:
+        return
+    if same_ok and out.data_ptr() == other.data_ptr() and out.dtype == other.dtype and out.shape == other.shape and (out.shape[0] == 1 or out.stride(0) == other.stride(0)):
+        return
+    a, b = _span(out), _span(other)
+    _need(a[1] <= b[0] or b[1] <= a[0], f"{what} overlaps an input without being it")
+
+
+def rmsnorm(x, w, *, res=None, fmt="same", h=None, rstd=None, eps=1e-6):
+    """Root-mean-square norm with the residual's addition (dist_op_rmsnorm): h = x + res, y = h / sqrt(mean h^2 + eps) * w over x [rows, C] (bf16 / fp32; w fp32).
+    fmt "same": y in x's type; "e4m3": bytes `q` and fp32 `scale` per row (what quant_rows_fp8 returns); "mxfp4": `codes` and `scales` (what quant_mxfp4 returns).
+    `h` is returned in x's type when `res` is given (or a buffer for it is: it may be x or res itself); `rstd` (fp32 [rows]) is filled when given, for rmsnorm_bwd.
+    Returns dict(y | q, scale | codes, scales [, h])."""
+    lib = L.load()
+    _need(fmt in RMS_FMTS, f"fmt {fmt!r}: one of {sorted(RMS_FMTS)}")
+    dt = _dt(x)
+    _need(x.dim() == 2 and x.shape[1] > 0, f"x: expected [rows, C] with C > 0, got {tuple(x.shape)}")
+    rows, Cc = x.shape
+    dev = x.device
+    a = L.RmsArgs()
+    a.ldx = _rows(x, rows, Cc, "x")
+    _vector(w, Cc, "w")
+    if rstd is not None:
+        _vector(rstd, rows, "rstd")
+    if res is not None:
+        a.ldres = _rows(res, rows, Cc, "res", x.dtype)
+    with _on_device(x, w, res, h, rstd):
+        out = {}
+        if h is None and res is not None:
+            h = torch.empty(rows, Cc, dtype=x.dtype, device=dev)
+        if h is not None:
+            a.ldh = _rows(h, rows, Cc, "h", x.dtype)
+            _apart(h, x, "h")
+            _apart(h, res, "h")
+            out["h"] = h
+        if fmt == "same":
+            out["y"] = y = torch.empty(rows, Cc, dtype=x.dtype, device=dev)
+        elif fmt == "e4m3":
+            out["q"] = y = torch.empty(rows, Cc, dtype=torch.uint8, device=dev)
+            out["scale"] = sc = torch.empty(rows, dtype=torch.float32, device=dev)
+            a.scale = sc.data_ptr()
+        else:
+            out["codes"], out["scales"] = y, sc = _mx_empty(rows, Cc, dev)
+            a.scale = sc.data_ptr()
+        a.x, a.w, a.y, a.ldy = x.data_ptr(), w.data_ptr(), y.data_ptr(), y.shape[1]
+        a.res, a.h, a.rstd = (res.data_ptr() if res is not None else None), (h.data_ptr() if h is not None else None), (rstd.data_ptr() if rstd is not None else None)
+        a.rows, a.C, a.fmt, a.dtype, a.eps = rows, Cc, RMS_FMTS[fmt], dt, eps
+        L.check(lib.dist_op_rmsnorm(C.byref(a), _stream()))
+    return out
+
+
+def rmsnorm_bwd(h, rstd, dy, w, *, dres=None, dh=None, dw=None):
+    """Backward of rmsnorm from its h and rstd (dist_op_rmsnorm_bwd); dy [rows, C] in bf16 or fp32, dres (h's type): the gradient that reaches h past the norm, added to dh.
+    dh: a buffer for the result (it may be dres, h or dy itself); dw (fp32 [C]) is ACCUMULATED into when given.  Returns (dh, dw).  The same bits every time."""
+    lib = L.load()
+    a = L.RmsBwdArgs()
+    a.dtype, a.dy_dtype = _dt(h), _dt(dy)
+    _need(h.dim() == 2 and h.shape[1] > 0, f"h: expected [rows, C] with C > 0, got {tuple(h.shape)}")
+    rows, Cc = h.shape
+    a.ldh, a.lddy = _rows(h, rows, Cc, "h"), _rows(dy, rows, Cc, "dy")
+    _vector(w, Cc, "w")
+    _vector(rstd, rows, "rstd")
+    if dres is not None:
+        a.lddres = _rows(dres, rows, Cc, "dres", h.dtype)
+    with _on_device(h, rstd, dy, w, dres, dh, dw):
+        if dh is None:
+            dh = torch.empty(rows, Cc, dtype=h.dtype, device=h.device)
+        a.lddh = _rows(dh, rows, Cc, "dh", h.dtype)
+        for t in (h, dy, dres):
+            _apart(dh, t, "dh")
+        a.accumulate = int(dw is not None)
+        if dw is None:
+            dw = torch.empty(Cc, dtype=torch.float32, device=h.device)
+        _vector(dw, Cc, "dw")
+        n = lib.dist_op_rmsnorm_bwd_scratch(rows, Cc)
+        scratch = torch.empty(n, dtype=torch.float32, device=h.device)
+        a.h, a.rstd, a.dy, a.w, a.dres = h.data_ptr(), rstd.data_ptr(), dy.data_ptr(), w.data_ptr(), (dres.data_ptr() if dres is not None else None)
+        a.dh, a.dw, a.scratch, a.scratch_elems, a.rows, a.C = dh.data_ptr(), dw.data_ptr(), scratch.data_ptr(), n, rows, Cc
+        L.check(lib.dist_op_rmsnorm_bwd(C.byref(a), _stream()))
+    return dh, dw
+
+
+def _mx_empty(rows, K, device):
+    """buffers of an MXFP4 operand of `rows` rows of K elements: (codes [rows, Kp / 2], scales [chunks, rows, 8]), uint8"""
+    return torch.empty(rows, (K + 31) // 32 * 16, dtype=torch.uint8, device=device), torch.empty((K + 255) // 256, rows, 8, dtype=torch.uint8, device=device)
+
+
+def _mx_operand(op, what):
+    """(codes, scales) as quant_mxfp4 returns them -> (rows, K)"""
+    _need(isinstance(op, (tuple, list)) and len(op) == 2, f"{what}: expected the pair that quant_mxfp4 returns")
+    codes, scales = op
+    _need(codes.dtype == torch.uint8 and codes.dim() == 2 and codes.is_contiguous() and codes.shape[1] > 0 and codes.shape[1] % 16 == 0,
+          f"{what}: codes must be contiguous uint8 [rows, K / 2], K a multiple of 32 (got {codes.dtype} {tuple(codes.shape)})")
+    rows, K = codes.shape[0], codes.shape[1] * 2
+    _need(scales.dtype == torch.uint8 and scales.is_contiguous() and tuple(scales.shape) == ((K + 255) // 256, rows, 8),
+          f"{what}: scales must be contiguous uint8 {((K + 255) // 256, rows, 8)} (got {scales.dtype} {tuple(scales.shape)})")
+    return rows, K
+
+
+def quant_mxfp4(x, *, transpose=False):
+    """x [rows, cols] (bf16 / fp32) in microscaled 4-bit floating point (dist_op_quant_mxfp4): (codes uint8 [rows, Kp / 2], scales uint8 [chunks, rows, 8]), blocks of 32 along
+    the columns; transpose=True: of x^T, codes [cols, Kp / 2], blocks along x's rows.  Kp is the length of the blocked axis rounded up to 32 (zeros behind it)."""
+    lib = L.load()
+    dt = _dt(x)
+    _need(x.dim() == 2, f"x: expected a matrix, got {tuple(x.shape)}")
+    rows, cols = x.shape
+    ld = _rows(x, rows, cols, "x")
+    n, K = (cols, rows) if transpose else (rows, cols)
+    _need(K > 0, "the quantised axis is empty")
+    with _on_device(x):
+        codes, scales = _mx_empty(n, K, x.device)
+        L.check(lib.dist_op_quant_mxfp4(x.data_ptr(), dt, rows, cols, ld, int(transpose), codes.data_ptr(), scales.data_ptr(), _stream()))
+    return codes, scales
+
+
+def dequant_mxfp4(codes, scales, dtype=torch.bfloat16):
+    """the values (codes, scales) of quant_mxfp4 stand for, [rows, Kp] in `dtype` (bf16 / fp32; exact) (dist_op_dequant_mxfp4)"""
+    lib = L.load()
+    rows, K = _mx_operand((codes, scales), "operand")
+    with _on_device(codes, scales):
+        y = torch.empty(rows, K, dtype=dtype, device=codes.device)
+        L.check(lib.dist_op_dequant_mxfp4(codes.data_ptr(), scales.data_ptr(), rows, K, y.data_ptr(), _dt(y), _stream()))
+    return y
+
+
+def gemm_mxfp4(A, B, *, bias=None, res=None, out=None, out_dtype=torch.bfloat16):
+    """C [M, N] = A B^T + bias + res with an MXFP4 weight (dist_op_gemm_mxfp4).  B: (codes, scales) from quant_mxfp4, N rows of K.  A: (codes, scales) likewise (also from
+    rmsnorm(fmt="mxfp4")), or (q uint8 [M, K], scale fp32 [M]) from rmsnorm(fmt="e4m3") / quant_rows_fp8.  bias fp32 [N]; res [M, N] in C's type (it may be `out` itself).
+    C is bf16, or fp32 with an MXFP4 A.  The gradients are the same call: dA = gemm_mxfp4(quant_mxfp4(dC), quant_mxfp4(W, transpose=True)),
+    dW = gemm_mxfp4(quant_mxfp4(dC, transpose=True), quant_mxfp4(X, transpose=True))."""
+    lib = L.load()
+    N, K = _mx_operand(B, "B")
+    _need(N > 0, "B has no rows")
+    _need(isinstance(A, (tuple, list)) and len(A) == 2, "A: expected a pair (codes, scales) or (q, scale)")
+    a = L.GemmMxArgs()
+    q, sc = A
+    if sc.dtype == torch.float32:
+        _need(q.dim() == 2 and q.shape[1] == K, f"A: expected [M, {K}] e4m3 bytes, got {tuple(q.shape)}")
+        M = q.shape[0]
+        lda = _rows(q, M, K, "A", torch.uint8)
+        _need(lda % 16 == 0 and q.data_ptr() % 16 == 0, "A: rows of e4m3 bytes must start at multiples of 16 bytes")
+        _vector(sc, M, "A's scale")
+        a.a_fmt, a.lda = L.MX_A_E4M3, lda
+    else:
+        M, Ka = _mx_operand(A, "A")
+        _need(Ka == K, f"A has {Ka} elements a row, B has {K}")
+        a.a_fmt = L.MX_A_MXFP4
+    with _on_device(B[0], B[1], q, sc, bias, res, out):
+        if out is None:
+            out = torch.empty(M, N, dtype=out_dtype, device=q.device)
+        elif M > 0:
+            _rows(out, M, N, "out")
+            for t in (q, B[0]):
+                _apart(out, t, "out", same_ok=False)
+        a.dtype = _dt(out)
+        _need(a.a_fmt == L.MX_A_MXFP4 or a.dtype == L.BF16, "a product with an e4m3 operand gives bf16")
+        a.ldc = _rows(out, M, N, "out")
+        if bias is not None:
+            _vector(bias, N, "bias")
+            a.bias = bias.data_ptr()
+        if res is not None:
+            a.res, a.ldres = res.data_ptr(), _rows(res, M, N, "res", out.dtype)
+            _apart(out, res, "out")
+        n = lib.dist_op_gemm_mxfp4_scratch(M, N, K, a.a_fmt)
+        if n > 0:
+            scratch = torch.empty(n, dtype=torch.float32, device=q.device)
+            a.scratch, a.scratch_elems = scratch.data_ptr(), n
+        a.A, a.a_scale, a.B, a.b_scale, a.C = q.data_ptr(), sc.data_ptr(), B[0].data_ptr(), B[1].data_ptr(), out.data_ptr()
+        a.M, a.N, a.K = M, N, K
+        L.check(lib.dist_op_gemm_mxfp4(C.byref(a), _stream()))
+    return out

@@ -1,0 +1,510 @@
+"""The norm, the MXFP4 quantisation and the MXFP4 product on the GPU against their definitions in 64 bits (tests/_mx_oracle.py).
+
+Tolerances, all derived: a rounding is off by at most half a step (`half`), an fp32 operation by U = 2^-24 of its result, a sum of n fp32 terms by (additions on the longest
+path) U times the sum of the terms' magnitudes."""
+import pytest
+import torch
+
+import _mx_oracle as mo
+from dist_amd import lib as L
+from dist_amd import ops
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+BF, F32 = torch.bfloat16, torch.float32
+half = mo.half
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def act(rows, C, dtype, seed, wide=False):
+    """activations with columns of different size; wide: a view into a wider buffer, rows neither adjacent nor 16-byte aligned"""
+    g = gen(seed)
+    x = (torch.randn(rows, C, generator=g) * torch.exp(0.7 * torch.randn(C, generator=g))).to(dtype)
+    if not wide:
+        return x.cuda()
+    buf = torch.full((rows, C + 5), float("nan"), dtype=dtype).cuda()
+    buf[:, 3:3 + C] = x.cuda()
+    return buf[:, 3:3 + C]
+
+
+def close(got, want, tol, what=""):
+    got, want = got.double().cpu(), want.double().cpu()
+    bad = ~((got - want).abs() <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((got - want).abs().max())}, first at {bad.nonzero()[0].tolist()}"
+
+
+def same_bits(a, b):
+    assert a.dtype == b.dtype and a.shape == b.shape
+    assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+
+# additions on the longest path of a row's sum: 128 elements in a lane (16384 / 256 in the widest, C / 256 for longer rows), 8 in the tree, and the operations around it
+def depth(C):
+    return max(64, C // 256) + 8 + 8
+
+
+WIDTHS = [1, 2, 7, 8, 31, 32, 33, 64, 200, 256, 384, 392, 768, 776, 1000, 1024, 1032, 1411, 2048, 2056, 2500, 4096, 4100, 4104, 8192, 8200]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("C", WIDTHS)
+def test_norm_every_width(C, dtype, gpu_lib):
+    rows = 5
+    x, r, w = act(rows, C, dtype, C), act(rows, C, dtype, C + 1), 1 + 0.2 * torch.randn(C, generator=gen(C + 2)).cuda()
+    if C > 1:
+        x[2], r[2] = 0, 0
+    rstd = torch.empty(rows, device="cuda")
+    n = ops.rmsnorm(x, w, res=r, rstd=rstd)
+    h, s, y = mo.rms(x, w, r)
+    rel = depth(C) * U
+    close(rstd, s, rel * s, "rstd")
+    close(n["h"], h, (half(dtype) + U) * h.abs(), "h")
+    close(n["y"], y, (half(dtype) + 2 * rel) * y.abs() + 1e-45, "y")
+    # the plain form without a residual reads x itself
+    same_bits(ops.rmsnorm(n["h"], w)["y"], ops.rmsnorm(n["h"].clone(), w)["y"])
+
+
+@pytest.mark.parametrize("C", [1, 31, 64, 200, 768, 1000, 1411, 2048, 4096, 4104, 8192, 8200])
+def test_norm_8_and_4_bits_are_the_quantised_norm(C, gpu_lib):
+    """in fp32 the unrounded y is the output y: its e4m3 and MXFP4 forms are bit for bit what the quantisers make of it"""
+    x, w = act(6, C, F32, C), 1 + 0.2 * torch.randn(C, generator=gen(C + 2)).cuda()
+    x[3] = 0
+    y = ops.rmsnorm(x, w)["y"]
+    q = ops.rmsnorm(x, w, fmt="mxfp4")
+    codes, scales = ops.quant_mxfp4(y)
+    same_bits(q["codes"], codes)
+    same_bits(q["scales"], scales)
+    e = ops.rmsnorm(x, w, fmt="e4m3")
+    a = y.abs().amax(1)
+    close(e["scale"], torch.where(a > 0, a / torch.full_like(a, 448), torch.ones_like(a)), 0.0, "scale")      # (a tensor: torch multiplies by 1 / 448 for a number)
+    want = (y * torch.where(a > 0, 448 / a, torch.ones_like(a))[:, None]).to(torch.float8_e4m3fn)
+    same_bits(e["q"], want.view(torch.uint8))
+    if C % 8 == 0 and C <= 8192:
+        q8, s8 = ops.quant_rows_fp8(y)
+        same_bits(e["q"], q8)
+        same_bits(e["scale"], s8)
+
+
+@pytest.mark.parametrize("rows,C", [(1, 1024), (3, 768), (197, 96), (4, 3000), (2, 20000)])
+def test_norm_8_and_4_bits_of_bf16(rows, C, gpu_lib):
+    x, r, w = act(rows, C, BF, C), act(rows, C, BF, C + 1), 1 + 0.2 * torch.randn(C, generator=gen(C + 2)).cuda()
+    h, s, y = mo.rms(x, w, r)
+    rel = 2 * depth(C) * U
+    e = ops.rmsnorm(x, w, res=r, fmt="e4m3")
+    scale = y.abs().amax(1) / 448
+    close(e["scale"], scale, (rel + U) * scale, "scale")
+    got = e["q"].view(torch.float8_e4m3fn).double().cpu() * e["scale"].double().cpu()[:, None]
+    # half a step of e4m3 (relative above 2^-6 of the scaled value, 2^-10 absolute below), and what moves a value across a border
+    close(got, y, (half(torch.float8_e4m3fn) + 3 * rel) * y.abs() + 2.0 ** -10 * scale[:, None], "values")
+    q = ops.rmsnorm(x, w, res=r, fmt="mxfp4")
+    same_bits(q["h"], e["h"])
+    got = mo.read((q["codes"], q["scales"]))[:, :C].abs()
+    a, b = (mo.values_of(*mo.codes_of(y * f))[:, :C].abs() for f in (1 - rel, 1 + rel))          # rounding is monotonous: the result lies between those of y (1 -+ rel)
+    assert bool(((got >= torch.minimum(a, b)) & (got <= torch.maximum(a, b))).all())
+
+
+def test_norm_in_place_strided_and_padded(gpu_lib):
+    """h in x's or res's own memory, column slices of wider buffers (no 16-byte alignment), rows that stay as they were"""
+    for C in (768, 1411, 5000):
+        for dtype in (BF, F32):
+            x, r, w = act(9, C, dtype, 3, wide=True), act(9, C, dtype, 4, wide=True), torch.rand(C, generator=gen(5)).cuda()
+            want = ops.rmsnorm(x.contiguous(), w, res=r.contiguous())
+            n = ops.rmsnorm(x, w, res=r)
+            tol = 2 * depth(C) * U
+            close(n["h"], want["h"], 0.0)
+            close(n["y"], want["y"].double(), (half(dtype) * 2 + tol) * want["y"].double().abs().cpu())       # (another kernel: the sums' order differs)
+            for which in (0, 1):
+                a, b = x.clone(), r.clone()
+                out = ops.rmsnorm(a, w, res=b, h=(a, b)[which])
+                assert out["h"] is (a, b)[which]
+                close(out["h"], want["h"], 0.0)
+                close((b, a)[which], (r, x)[which], 0.0)
+            buf = torch.full((12, C), 7.0, dtype=dtype, device="cuda")
+            ops.rmsnorm(x, w, res=r, h=buf[:9])
+            close(buf[:9], want["h"], 0.0)
+            assert bool((buf[9:] == 7).all())
+    x = act(4, 64, BF, 1)
+    wide = torch.zeros(5, 64, dtype=BF, device="cuda")
+    with pytest.raises(L.DistError, match="overlaps"):
+        ops.rmsnorm(wide[:4], torch.ones(64, device="cuda"), res=x, h=wide[1:])
+
+
+def test_norm_not_a_number_stays_in_its_row(gpu_lib):
+    for C in (768, 1411, 5000):
+        x, w = act(4, C, BF, 1), torch.ones(C, device="cuda")
+        x[1, 5], x[2, 7] = float("nan"), float("inf")
+        clean = act(4, C, BF, 1)
+        for fmt in ("same", "e4m3", "mxfp4"):
+            n, ok = ops.rmsnorm(x, w, fmt=fmt), ops.rmsnorm(clean, w, fmt=fmt)
+            val = {"same": lambda n: n["y"].float(), "e4m3": lambda n: n["q"].view(torch.float8_e4m3fn).float() * n["scale"][:, None],
+                   "mxfp4": lambda n: ops.dequant_mxfp4(n["codes"], n["scales"], F32)[:, :C]}[fmt]
+            v, o = val(n), val(ok)
+            assert bool(v[1].isnan().all()) and bool(v[2].isnan().any())
+            close(v[[0, 3]], o[[0, 3]], 0.0)
+
+
+@pytest.mark.parametrize("dtype,dyt", [(BF, BF), (BF, F32), (F32, F32), (F32, BF)])
+@pytest.mark.parametrize("C", [1, 8, 33, 96, 384, 768, 1000, 1024, 1411, 2048, 2056, 4096, 4100, 8192, 8200])
+def test_norm_gradient(C, dtype, dyt, gpu_lib):
+    rows = 37
+    h, d, r, w = act(rows, C, dtype, C), act(rows, C, dyt, C + 1), act(rows, C, dtype, C + 2), 1 + 0.2 * torch.randn(C, generator=gen(C)).cuda()
+    rstd = mo.rms(h, w)[1].float().cuda()
+    dh, dw = ops.rmsnorm_bwd(h, rstd, d, w, dres=r)
+    want, wantw = mo.rms_bwd(h, rstd, d, w, r)
+    n, g = h.double().cpu() * rstd.double().cpu()[:, None], d.double().cpu() * w.double().cpu()
+    mean = (g * n).abs().mean(1, keepdim=True)
+    m = (g * n).mean(1, keepdim=True).abs()
+    inner = rstd.double().cpu()[:, None] * (4 * g.abs() + n.abs() * ((depth(C) + 4) * mean + 6 * m)) + 2 * r.double().cpu().abs()
+    close(dh, want, half(dtype) * want.abs() + 1.01 * U * inner, "dh")
+    # a column's sum: at most 37 rows in one block's chain, 16 slots, 64 partial rows and 16 groups
+    close(dw, wantw, (37 + 16 + 64 + 16 + 4) * U * (d.double().cpu() * n).abs().sum(0), "dw")
+    dh2, dw2 = ops.rmsnorm_bwd(h, rstd, d, w, dres=r)
+    same_bits(dh, dh2)
+    same_bits(dw, dw2)
+    acc = torch.full((C,), 3.0, device="cuda")
+    ops.rmsnorm_bwd(h, rstd, d, w, dw=acc)
+    close(acc, dw.double().cpu() + 3, 2 * U * (dw.double().cpu().abs() + 3), "accumulated")
+    for buf in [h, r] + ([d] if dyt == dtype else []):               # in place
+        c = [t.clone() for t in (h, d, r)]
+        out = c[[t is buf for t in (h, d, r)].index(True)]
+        same_bits(ops.rmsnorm_bwd(c[0], rstd, c[1], w, dres=c[2], dh=out)[0], dh)
+
+
+def test_norm_gradient_many_rows_and_none(gpu_lib):
+    for rows, C, dt in ((9001, 768, BF), (4999, 100, F32), (70, 9000, BF)):
+        h, d, w = act(rows, C, dt, 1), act(rows, C, dt, 2), torch.rand(C, generator=gen(3)).cuda()
+        rstd = mo.rms(h, w)[1].float().cuda()
+        dh, dw = ops.rmsnorm_bwd(h, rstd, d, w)
+        want, wantw = mo.rms_bwd(h, rstd, d, w)
+        n = h.double().cpu() * rstd.double().cpu()[:, None]
+        close(dw, wantw, (200 + rows // 256) * U * (d.double().cpu() * n).abs().sum(0), "dw")
+        rel = float((dh.double().cpu() - want).norm() / want.norm())
+        assert rel <= half(dt) + 1e-6
+    h0 = torch.empty(0, 64, dtype=BF, device="cuda")
+    dh, dw = ops.rmsnorm_bwd(h0, torch.empty(0, device="cuda"), h0, torch.ones(64, device="cuda"))
+    assert dh.shape == (0, 64) and bool((dw == 0).all())
+    assert ops.rmsnorm(h0, torch.ones(64, device="cuda"), fmt="e4m3")["q"].shape == (0, 64)
+
+
+# ---- quantisation ---------------------------------------------------------------------------------------------------------------------------------------------
+
+def spread(rows, K, dtype, seed):
+    """values over the whole range of exponents, exact ties, zeros and whole zero blocks"""
+    g = gen(seed)
+    x = torch.randn(rows, K, generator=g) * torch.exp2(torch.randint(-60, 60, (rows, 1), generator=g).float())
+    grid = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, 6.0, 0.0, -0.25, -2.5, -5.0])
+    pick = torch.randint(0, 13, (rows, K), generator=g)
+    x = torch.where(torch.rand(rows, K, generator=g) < 0.3, grid[pick], x)
+    x[torch.rand(rows, K, generator=g) < 0.05] = 0
+    if rows > 2:
+        x[1] = 0
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,K", [(1, 1), (1, 32), (2, 31), (5, 33), (3, 64), (7, 200), (4, 255), (4, 256), (4, 257), (9, 288), (33, 1000), (65, 1024), (2, 8200)])
+def test_quant_rows_and_columns(rows, K, dtype, gpu_lib):
+    x = spread(rows, K, dtype, rows * 1000 + K)
+    code, byte = mo.codes_of(x)
+    want = mo.pack(code, byte)
+    got = ops.quant_mxfp4(x.cuda())
+    same_bits(got[0].cpu(), want[0])
+    same_bits(got[1].cpu(), want[1])
+    buf = torch.full((rows, K + 3), float("nan"), dtype=dtype, device="cuda")
+    buf[:, 1:K + 1] = x.cuda()
+    strided = ops.quant_mxfp4(buf[:, 1:K + 1])
+    same_bits(strided[0], got[0])
+    same_bits(strided[1], got[1])
+    t = ops.quant_mxfp4(x.t().contiguous().cuda(), transpose=True)                 # the same operand from its transpose
+    same_bits(t[0], got[0])
+    same_bits(t[1], got[1])
+    for out in (BF, F32):
+        back = ops.dequant_mxfp4(*got, dtype=out)
+        close(back, mo.values_of(code, byte), 0.0, "read back")
+
+
+def test_quant_every_bf16_value_and_the_ends_of_fp32(gpu_lib):
+    """every finite bf16 beside a block maximum of each exponent is rounded as the definition says; fp32 values next to the borders and at both ends of the range"""
+    every = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(BF)
+    every = every[torch.isfinite(every)].view(-1, 16)                              # 16 neighbours and, next to them, a larger maximum
+    for lift in (0, 1, 4):
+        x = torch.zeros(every.shape[0], 32, dtype=F32)
+        x[:, :16] = every.float()
+        x[:, 16] = every.float().abs().amax(1) * 2.0 ** lift
+        x = torch.where(torch.isfinite(x), x, torch.zeros_like(x)).to(BF)
+        got = ops.quant_mxfp4(x.cuda())
+        want = mo.pack(*mo.codes_of(x))
+        same_bits(got[0].cpu(), want[0])
+        same_bits(got[1].cpu(), want[1])
+    tiny, big = 2.0 ** -149, float(torch.finfo(F32).max)
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0])
+    x = torch.zeros(40, 32)
+    for i in range(32):
+        x[i, 0] = 6.0 * 2.0 ** (i - 16)
+        x[i, 1:10] = borders * 2.0 ** (i - 16)
+        x[i, 10:19] = torch.nextafter(borders, torch.tensor(0.0)) * 2.0 ** (i - 16)
+        x[i, 19:28] = torch.nextafter(borders, torch.tensor(9.0)) * 2.0 ** (i - 16)
+    x[32, :5] = torch.tensor([tiny, -tiny, 3 * tiny, 2.0 ** -126, 2.0 ** -127])
+    x[33, :3] = torch.tensor([tiny, 0.0, -0.0])
+    x[34, :3] = torch.tensor([big, -big, big / 3])
+    x[35, :3] = torch.tensor([2.0 ** -125, 2.0 ** -126, 2.0 ** -128])
+    x[36, 3], x[37, 4], x[38, 5] = float("inf"), float("-inf"), float("nan")
+    got = ops.quant_mxfp4(x.cuda())
+    want = mo.pack(*mo.codes_of(x))
+    same_bits(got[0].cpu(), want[0])
+    same_bits(got[1].cpu(), want[1])
+    back = ops.dequant_mxfp4(*got, dtype=F32)
+    assert bool(back[36:39].isnan().all()) and not bool(back[:36].isnan().any())
+    t = ops.quant_mxfp4(x.t().contiguous().cuda(), transpose=True)
+    same_bits(t[0], got[0])
+    same_bits(t[1], got[1])
+
+
+# ---- product --------------------------------------------------------------------------------------------------------------------------------------------------
+
+def operand(rows, K, seed):
+    g = gen(seed)
+    code = torch.randint(0, 16, (rows, -(-K // 32) * 32), generator=g)
+    byte = 127 + torch.randint(-6, 4, (rows, code.shape[1] // 32), generator=g)
+    q, sc = mo.pack(code, byte)
+    return (q.cuda(), sc.cuda()), mo.values_of(code, byte)
+
+
+def rows8(M, K, seed):
+    x = act(M, K, F32, seed)
+    a = x.abs().amax(1, keepdim=True)
+    q = (x * (448 / a)).to(torch.float8_e4m3fn)
+    scale = (a / 448)[:, 0].contiguous()
+    return (q.view(torch.uint8), scale), q.double().cpu() * scale.double().cpu()[:, None]
+
+
+def check_product(M, N, K, fmt, out, bias, res, seed=0):
+    B, b = operand(N, K, seed + 1)
+    A, a = operand(M, K, seed + 2) if fmt == "mxfp4" else rows8(M, K, seed + 2)
+    g = gen(seed + 3)
+    bi = torch.randn(N, generator=g).cuda() if bias else None
+    r = torch.randn(M, N, generator=g).to(out).cuda() if res else None
+    c = ops.gemm_mxfp4(A, B, bias=bi, res=r, out_dtype=out)
+    assert c.dtype == out and c.shape == (M, N)
+    want = a @ b.t()
+    mag = a.abs() @ b.abs().t()
+    extra = torch.zeros_like(want)
+    for t in (bi, r):
+        if t is not None:
+            want = want + t.double().cpu()
+            extra = extra + t.double().cpu().abs()
+    # K / 32 block sums and their additions, in fp32; an e4m3 operand's products are aligned to the largest of eight with 13 bits below it: eight times 2^-13 of it, and the
+    # largest is at most the sum of the eight
+    tol = (K // 32 + 16) * U * mag + 3 * U * (mag + extra) + half(out) * want.abs() + (2.0 ** -10 * mag if fmt == "e4m3" else 0)
+    close(c, want, tol, f"{M}x{N}x{K} {fmt}")
+    if fmt == "e4m3":
+        assert float((c.double().cpu() - want).norm() / want.norm()) <= half(BF)
+    same_bits(c, ops.gemm_mxfp4(A, B, bias=bi, res=r, out_dtype=out))              # the same bits every time
+    return c
+
+
+@pytest.mark.parametrize("K", [32, 64, 96, 128, 160, 224, 256, 288, 384, 416, 512, 544, 1024, 1056])
+@pytest.mark.parametrize("fmt", ["mxfp4", "e4m3"])
+def test_product_every_tail_of_k(K, fmt, gpu_lib):
+    for M, N in ((1, 17), (40, 64), (130, 100)):
+        check_product(M, N, K, fmt, BF, True, True, K)
+
+
+@pytest.mark.parametrize("M", [1, 2, 8, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 127, 128, 129, 197, 255, 256, 257, 300])
+def test_product_every_height(M, gpu_lib):
+    for N, K, fmt, out in ((96, 288, "mxfp4", F32), (96, 288, "mxfp4", BF), (64, 384, "e4m3", BF)):
+        check_product(M, N, K, fmt, out, M % 2 == 0, M % 3 == 0, M)
+
+
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 7, 8, 15, 16, 17, 24, 33, 63, 64, 65, 100, 127, 128, 129, 200, 255, 256, 257, 512, 776])
+def test_product_every_width(N, gpu_lib):
+    for M, K, fmt, out in ((5, 96, "mxfp4", F32), (150, 160, "mxfp4", BF), (20, 320, "e4m3", BF), (270, 544, "e4m3", BF), (3, 2048, "mxfp4", F32)):
+        check_product(M, N, K, fmt, out, N % 2 == 0, N % 3 == 0, N)
+
+
+@pytest.mark.parametrize("M,N,K,fmt,out", [(1, 4096, 1024, "e4m3", BF), (1, 2304, 768, "mxfp4", F32), (16, 4096, 4096, "mxfp4", BF), (64, 768, 4096, "e4m3", BF), (1576, 768, 768, "mxfp4", BF),
+                                           (2600, 2304, 768, "mxfp4", BF), (1028, 1024, 4096, "e4m3", BF), (768, 768, 6304, "mxfp4", F32), (300, 200, 16384, "mxfp4", F32), (4100, 520, 1056, "e4m3", BF),
+                                           (513, 1411, 416, "mxfp4", F32), (130, 4095, 128, "e4m3", BF), (20000, 64, 96, "mxfp4", BF)])
+def test_product_sizes_of_use(M, N, K, fmt, out, gpu_lib):
+    check_product(M, N, K, fmt, out, True, True, 5)
+
+
+def test_product_into_buffers(gpu_lib):
+    """out and res as columns of wider buffers, at any alignment; rows behind the last one and columns beside it stay as they were; res in out's own memory"""
+    for M, N, K in ((5, 64, 96), (70, 129, 288), (300, 256, 256)):
+        for out in (BF, F32):
+            B, A = operand(N, K, 1)[0], operand(M, K, 2)[0]
+            bias = torch.randn(N, generator=gen(3)).cuda()
+            res = torch.randn(M, N, generator=gen(4)).to(out).cuda()
+            want = ops.gemm_mxfp4(A, B, bias=bias, res=res, out_dtype=out)
+            for off in (0, 1, 8):
+                buf = torch.full((M + 2, N + 16), 7.0, dtype=out, device="cuda")
+                keep = buf.clone()
+                view = buf[1:M + 1, off:off + N]
+                got = ops.gemm_mxfp4(A, B, bias=bias, res=res, out=view)
+                assert got is view
+                same_bits(view, want)
+                buf[1:M + 1, off:off + N] = 7.0
+                assert torch.equal(buf, keep)
+                view.copy_(res)
+                ops.gemm_mxfp4(A, B, bias=bias, res=view, out=view)
+                same_bits(view, want)
+            bias1 = torch.zeros(N + 1, device="cuda")[1:]
+            bias1.copy_(bias)
+            same_bits(ops.gemm_mxfp4(A, B, bias=bias1, res=res, out_dtype=out), want)
+    q = torch.zeros(4, 64, dtype=torch.uint8, device="cuda")
+    with pytest.raises(L.DistError, match="16 bytes"):
+        ops.gemm_mxfp4((torch.zeros(4, 72, dtype=torch.uint8, device="cuda")[:, :64], torch.ones(4, device="cuda")), operand(8, 64, 1)[0])
+    with pytest.raises(L.DistError, match="bf16"):
+        ops.gemm_mxfp4((q, torch.ones(4, device="cuda")), operand(8, 64, 1)[0], out_dtype=F32)
+    wide = torch.zeros(4, 80, dtype=torch.uint8, device="cuda")
+    wide[:, :64] = rows8(4, 64, 1)[0][0]
+    A = (wide[:, :64], torch.ones(4, device="cuda"))
+    same_bits(ops.gemm_mxfp4(A, operand(8, 64, 1)[0]), ops.gemm_mxfp4((A[0].contiguous(), A[1]), operand(8, 64, 1)[0]))
+
+
+def test_product_not_a_number_stays_in_its_row_and_column(gpu_lib):
+    for M, N, K in ((3, 40, 96), (80, 140, 288), (300, 300, 512)):
+        x, y = act(M, K, F32, 1), act(N, K, F32, 2)
+        x[1, 40], y[33, 70] = float("nan"), float("inf")
+        c = ops.gemm_mxfp4(ops.quant_mxfp4(x), ops.quant_mxfp4(y), out_dtype=F32)
+        nan = torch.zeros(M, N, dtype=torch.bool, device="cuda")
+        nan[1], nan[:, 33] = True, True
+        assert torch.equal(c.isnan(), nan)
+        e = rows8(M, K, 1)[0]
+        e[0][1, 40] = 0x7f                                                # e4m3's NaN
+        c = ops.gemm_mxfp4(e, ops.quant_mxfp4(act(N, K, F32, 2)))
+        assert bool(c[1].isnan().all()) and not bool(c[[0, 2]].isnan().any())
+
+
+def test_empty_products(gpu_lib):
+    B = operand(8, 64, 1)[0]
+    for A in ((torch.empty(0, 32, dtype=torch.uint8, device="cuda"), torch.empty(1, 0, 8, dtype=torch.uint8, device="cuda")), (torch.empty(0, 64, dtype=torch.uint8, device="cuda"), torch.empty(0, device="cuda"))):
+        assert ops.gemm_mxfp4(A, B, bias=torch.ones(8, device="cuda")).shape == (0, 8)
+    assert ops.quant_mxfp4(torch.empty(0, 64, device="cuda"))[0].shape == (0, 32)
+    assert ops.dequant_mxfp4(*ops.quant_mxfp4(torch.empty(0, 64, device="cuda"))).shape == (0, 64)
+
+
+# ---- far offsets, streams, graphs, the run of them together -------------------------------------------------------------------------------------------------------
+
+def test_offsets_past_32_bits(gpu_lib):
+    """outputs and inputs of more than 2^32 bytes and 2^31 elements: the last rows are those of a small call"""
+    C = 2048
+    rows = (1 << 31) // C + 3
+    w = torch.rand(C, generator=gen(1)).cuda()
+    x = torch.zeros(rows, C, dtype=BF, device="cuda")
+    tail = act(3, C, BF, 2)
+    x[-3:] = tail
+    small = ops.rmsnorm(tail, w, fmt="e4m3")
+    n = ops.rmsnorm(x, w, fmt="e4m3")
+    same_bits(n["q"][-3:], small["q"])
+    c = ops.gemm_mxfp4((n["q"], n["scale"]), operand(64, C, 3)[0])
+    same_bits(c[-3:], ops.gemm_mxfp4((small["q"], small["scale"]), operand(64, C, 3)[0]))
+    del n, c
+    q, ref = ops.quant_mxfp4(x), ops.quant_mxfp4(tail)
+    same_bits(q[0][-3:], ref[0])
+    same_bits(q[1][:, -3:], ref[1])
+    y = ops.dequant_mxfp4(*q)
+    same_bits(y[-3:], ops.dequant_mxfp4(*ref))
+    del y, x
+    B = operand(C, C, 4)[0]
+    c = ops.gemm_mxfp4(q, B)
+    same_bits(c[-3:], ops.gemm_mxfp4(ref, B))
+    assert bool((c[-4] == 0).all())
+
+
+def layer(x, r, w, W, WT, bias, d, dres):
+    """norm + 4-bit product forward, then its input gradient: as a training step through a frozen layer runs them"""
+    rstd = torch.empty(x.shape[0], device="cuda")
+    n = ops.rmsnorm(x, w, res=r, fmt="e4m3", rstd=rstd)
+    z = ops.gemm_mxfp4((n["q"], n["scale"]), W, bias=bias)
+    dy = ops.gemm_mxfp4(ops.quant_mxfp4(d), WT, out_dtype=F32)
+    dx, dw = ops.rmsnorm_bwd(n["h"], rstd, dy, w, dres=dres)
+    return z, n["h"], dx, dw
+
+
+def layer_state(rows, C, N, seed):
+    W = torch.randn(N, C, generator=gen(seed)).cuda() * C ** -0.5
+    return [act(rows, C, BF, seed + 1), act(rows, C, BF, seed + 2), torch.rand(C, generator=gen(seed)).cuda() + 0.5, ops.quant_mxfp4(W), ops.quant_mxfp4(W, transpose=True),
+            torch.randn(N, generator=gen(seed + 3)).cuda(), act(rows, N, BF, seed + 4), act(rows, C, BF, seed + 5)]
+
+
+@pytest.mark.parametrize("rows,C,N", [(1, 96, 64), (197, 768, 200), (600, 256, 2304)])
+def test_layer_and_its_gradients_together(rows, C, N, gpu_lib):
+    s = layer_state(rows, C, N, 7)
+    x, r, w, W, WT, bias, d, dres = s
+    z, hb, dx, dw = layer(*s)
+    h, rstd, y = mo.rms(x, w, r)
+    # forward: e4m3 rounding (2^-4 of a value, uniform: below 2^-5 of the norm) and bf16's; the weight's values are the quantised ones
+    zw = y @ mo.read(W)[:, :C].t() + bias.double().cpu()
+    prod = (y @ mo.read(W)[:, :C].t())
+    assert float((z.double().cpu() - zw).norm()) <= 2.0 ** -5 * float((y.norm(dim=1)[:, None] * mo.read(W)[:, :C].norm(dim=1)[None]).norm()) + half(BF) * float(zw.norm()), prod.norm()
+    dq = mo.values_of(*mo.codes_of(d))
+    wt = mo.read(WT)
+    want, wantw = mo.rms_bwd(hb, rstd, dq[:, :N] @ wt[:, :N].t(), w, dres)
+    # d and W are rounded to 4 bits before the product on both sides: what is left is fp32 and the output's rounding; rstd comes from the unrounded h: U of it
+    assert float((dx.double().cpu() - want).norm()) <= (half(BF) + 64 * U) * float(want.norm())
+    mag = (dq[:, :N].abs() @ wt[:, :N].abs().t() * (hb.double().cpu() * rstd[:, None]).abs()).sum(0)
+    close(dw, wantw, (N // 32 + 16 + 200 + rows // 256 + 80) * U * mag, "dw")
+    # the weight's own gradient: the same product on the transposed operands, blocks along the tokens
+    dW = ops.gemm_mxfp4(ops.quant_mxfp4(d, transpose=True), ops.quant_mxfp4(hb, transpose=True), out_dtype=F32)
+    a, b = mo.values_of(*mo.codes_of(d.t())), mo.values_of(*mo.codes_of(hb.t()))
+    close(dW, a @ b.t(), (a.shape[1] // 32 + 24) * U * (a.abs() @ b.abs().t()), "dW")
+
+
+def test_other_stream_and_two_graphs(gpu_lib):
+    """captured and replayed among eager calls of the same operators on other data, two graphs alive at once; every replay gives the eager bits"""
+    sets = [layer_state(300, 256, 192, 11), layer_state(300, 256, 192, 23)]
+    want = [layer(*s) for s in sets]
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        got = layer(*sets[0])
+    torch.cuda.current_stream().wait_stream(st)
+    for a, b in zip(got, want[0]):
+        same_bits(a, b)
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(layer(*s))
+        graphs.append(g)
+    for k in (0, 1, 1, 0, 0, 1):
+        for t in outs[k]:
+            t.zero_()
+        graphs[k].replay()
+        eager = layer(*sets[1 - k])
+        torch.cuda.synchronize()
+        for a, b in zip(outs[k], want[k]):
+            same_bits(a, b)
+        for a, b in zip(eager, want[1 - k]):
+            same_bits(a, b)
+    # new inputs in the captured tensors
+    fresh = layer_state(300, 256, 192, 31)
+    for dst, src in zip(sets[0], fresh):
+        for u, v in zip(dst, src) if isinstance(dst, tuple) else [(dst, src)]:
+            u.copy_(v)
+    graphs[0].replay()
+    for a, b in zip(outs[0], layer(*fresh)):
+        same_bits(a, b)
+
+
+def test_two_streams_at_once(gpu_lib):
+    sets = [layer_state(500, 512, 384, 41), layer_state(500, 512, 384, 53)]
+    want = [layer(*s) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(layer(*sets[k]))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for g in got[k]:
+            for a, b in zip(g, want[k]):
+                same_bits(a, b)
