@@ -550,132 +550,70 @@ def attention_fp8(qkv8, in_scale, frames, Ltok, heads, out8_scale=None, amax=Non
 
 
 # ---- a 4-bit frozen linear layer: norm, microscaled 4-bit quantisation, product ---------------------------------------------------------------------------------
-class _NoGuard:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *_):
-        return False
-
-
-_NO_GUARD = _NoGuard()
+# (One token's call is bound by this host code: checks are plain comparisons, messages are made only when one fails, and the launch takes the raw stream of the
+# operands' GPU - 0.1 us against 2.8 us for torch.cuda.current_stream().)
 RMS_FMTS = {"same": L.RMS_SAME, "e4m3": L.RMS_E4M3, "mxfp4": L.RMS_MXFP4}
 
 
-def _need(ok, what):
-    if not ok:
-        raise L.DistError(what)
+def _refuse(what):
+    raise L.DistError(what)
 
 
-def _on_device(first, *others):
-    """every tensor on the GPU of `first`; returns the context in which the launch happens (that GPU current, so its current stream is the one used)"""
-    dev = first.device
-    _need(first.is_cuda, "the operands must be GPU tensors")
+def _device(first, *others):
+    """the index of the GPU that every operand is on"""
+    dev = first.get_device()
+    if dev < 0:
+        _refuse("the operands must be GPU tensors")
     for t in others:
-        _need(t is None or t.device == dev, f"operands on different devices: {dev} and {t.device if t is not None else None}")
-    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+        if t is not None and t.get_device() != dev:
+            _refuse(f"operands on different devices: {first.device} and {t.device}")
+    return dev
 
 
-def _rows(t, rows, cols, what, dtype=None):
-    """a [rows, cols] tensor whose rows are contiguous and do not overlap; returns the row pitch in elements"""
-    _need(t.dim() == 2 and t.shape[0] == rows and t.shape[1] == cols, f"{what}: expected shape {(rows, cols)}, got {tuple(t.shape)}")
-    _need(dtype is None or t.dtype == dtype, f"{what}: expected {dtype}, got {t.dtype}")
-    ld = t.stride(0) if rows > 1 else cols
-    _need((cols == 1 or t.stride(1) == 1) and ld >= cols, f"{what}: rows must be contiguous and must not overlap (strides {t.stride()})")
+def _launch(dev, fn, *args):
+    """on the operands' GPU, on its current stream"""
+    if dev == torch._C._cuda_getDevice():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if code != 0:
+        L.check(code)
+
+
+def _matrix(t, shape, what, dtype):
+    """a matrix of this shape and type whose rows are contiguous and do not overlap; returns the row pitch in elements"""
+    if t.dtype != dtype or t.shape != shape:
+        _refuse(f"{what}: expected {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    ld, step = t.stride()
+    rows, cols = shape
+    if rows < 2:
+        ld = cols
+    if (step != 1 and cols > 1) or ld < cols:
+        _refuse(f"{what}: rows must be contiguous and must not overlap (strides {t.stride()})")
     return ld
 
 
-def _vector(t, n, what, dtype=torch.float32):
-    _need(t.dtype == dtype and t.numel() == n and t.is_contiguous(), f"{what}: expected {n} contiguous {dtype} values, got {t.dtype} {tuple(t.shape)}")
+def _vector(t, n, what):
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        _refuse(f"{what}: expected {n} contiguous float32 values, got {t.dtype} {tuple(t.shape)}")
 
 
-def _span(t):
-    """first and last byte address of a [rows, cols] tensor"""
-    return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+def _apart(out, what, *inputs, may_be=True):
+    """an output that the caller brings may be one of the inputs itself (same address, type, shape and pitch) but must not overlap them otherwise"""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
 
-
-def _apart(out, other, what, same_ok=True):
-    """an output may be one of its inputs itself (same address, pitch and type) but must not overlap it otherwise"""
-    if out is None or other is None or out.numel() == 0 or other.numel() == 0:
+    if out.numel() == 0:
         return
-    if same_ok and out.data_ptr() == other.data_ptr() and out.dtype == other.dtype and out.shape == other.shape and (out.shape[0] == 1 or out.stride(0) == other.stride(0)):
-        return
-    a, b = _span(out), _span(other)
-    _need(a[1] <= b[0] or b[1] <= a[0], f"{what} overlaps an input without being it")
-
-
-def rmsnorm(x, w, *, res=None, fmt="same", h=None, rstd=None, eps=1e-6):
-    """Root-mean-square norm with the residual's addition (dist_op_rmsnorm): h = x + res, y = h / sqrt(mean h^2 + eps) * w over x [rows, C] (bf16 / fp32; w fp32).
-    fmt "same": y in x's type; "e4m3": bytes `q` and fp32 `scale` per row (what quant_rows_fp8 returns); "mxfp4": `codes` and `scales` (what quant_mxfp4 returns).
-    `h` is returned in x's type when `res` is given (or a buffer for it is: it may be x or res itself); `rstd` (fp32 [rows]) is filled when given, for rmsnorm_bwd.
-    Returns dict(y | q, scale | codes, scales [, h])."""
-    lib = L.load()
-    _need(fmt in RMS_FMTS, f"fmt {fmt!r}: one of {sorted(RMS_FMTS)}")
-    dt = _dt(x)
-    _need(x.dim() == 2 and x.shape[1] > 0, f"x: expected [rows, C] with C > 0, got {tuple(x.shape)}")
-    rows, Cc = x.shape
-    dev = x.device
-    a = L.RmsArgs()
-    a.ldx = _rows(x, rows, Cc, "x")
-    _vector(w, Cc, "w")
-    if rstd is not None:
-        _vector(rstd, rows, "rstd")
-    if res is not None:
-        a.ldres = _rows(res, rows, Cc, "res", x.dtype)
-    with _on_device(x, w, res, h, rstd):
-        out = {}
-        if h is None and res is not None:
-            h = torch.empty(rows, Cc, dtype=x.dtype, device=dev)
-        if h is not None:
-            a.ldh = _rows(h, rows, Cc, "h", x.dtype)
-            _apart(h, x, "h")
-            _apart(h, res, "h")
-            out["h"] = h
-        if fmt == "same":
-            out["y"] = y = torch.empty(rows, Cc, dtype=x.dtype, device=dev)
-        elif fmt == "e4m3":
-            out["q"] = y = torch.empty(rows, Cc, dtype=torch.uint8, device=dev)
-            out["scale"] = sc = torch.empty(rows, dtype=torch.float32, device=dev)
-            a.scale = sc.data_ptr()
-        else:
-            out["codes"], out["scales"] = y, sc = _mx_empty(rows, Cc, dev)
-            a.scale = sc.data_ptr()
-        a.x, a.w, a.y, a.ldy = x.data_ptr(), w.data_ptr(), y.data_ptr(), y.shape[1]
-        a.res, a.h, a.rstd = (res.data_ptr() if res is not None else None), (h.data_ptr() if h is not None else None), (rstd.data_ptr() if rstd is not None else None)
-        a.rows, a.C, a.fmt, a.dtype, a.eps = rows, Cc, RMS_FMTS[fmt], dt, eps
-        L.check(lib.dist_op_rmsnorm(C.byref(a), _stream()))
-    return out
-
-
-def rmsnorm_bwd(h, rstd, dy, w, *, dres=None, dh=None, dw=None):
-    """Backward of rmsnorm from its h and rstd (dist_op_rmsnorm_bwd); dy [rows, C] in bf16 or fp32, dres (h's type): the gradient that reaches h past the norm, added to dh.
-    dh: a buffer for the result (it may be dres, h or dy itself); dw (fp32 [C]) is ACCUMULATED into when given.  Returns (dh, dw).  The same bits every time."""
-    lib = L.load()
-    a = L.RmsBwdArgs()
-    a.dtype, a.dy_dtype = _dt(h), _dt(dy)
-    _need(h.dim() == 2 and h.shape[1] > 0, f"h: expected [rows, C] with C > 0, got {tuple(h.shape)}")
-    rows, Cc = h.shape
-    a.ldh, a.lddy = _rows(h, rows, Cc, "h"), _rows(dy, rows, Cc, "dy")
-    _vector(w, Cc, "w")
-    _vector(rstd, rows, "rstd")
-    if dres is not None:
-        a.lddres = _rows(dres, rows, Cc, "dres", h.dtype)
-    with _on_device(h, rstd, dy, w, dres, dh, dw):
-        if dh is None:
-            dh = torch.empty(rows, Cc, dtype=h.dtype, device=h.device)
-        a.lddh = _rows(dh, rows, Cc, "dh", h.dtype)
-        for t in (h, dy, dres):
-            _apart(dh, t, "dh")
-        a.accumulate = int(dw is not None)
-        if dw is None:
-            dw = torch.empty(Cc, dtype=torch.float32, device=h.device)
-        _vector(dw, Cc, "dw")
-        n = lib.dist_op_rmsnorm_bwd_scratch(rows, Cc)
-        scratch = torch.empty(n, dtype=torch.float32, device=h.device)
-        a.h, a.rstd, a.dy, a.w, a.dres = h.data_ptr(), rstd.data_ptr(), dy.data_ptr(), w.data_ptr(), (dres.data_ptr() if dres is not None else None)
-        a.dh, a.dw, a.scratch, a.scratch_elems, a.rows, a.C = dh.data_ptr(), dw.data_ptr(), scratch.data_ptr(), n, rows, Cc
-        L.check(lib.dist_op_rmsnorm_bwd(C.byref(a), _stream()))
-    return dh, dw
+    for t in inputs:
+        if t is None or t.numel() == 0:
+            continue
+        if may_be and out.data_ptr() == t.data_ptr() and out.dtype == t.dtype and out.shape == t.shape and (out.shape[0] == 1 or out.stride(0) == t.stride(0)):
+            continue
+        a, b = span(out), span(t)
+        if a[0] < b[1] and b[0] < a[1]:
+            _refuse(f"{what} overlaps an input without being it")
 
 
 def _mx_empty(rows, K, device):
@@ -685,39 +623,115 @@ def _mx_empty(rows, K, device):
 
 def _mx_operand(op, what):
     """(codes, scales) as quant_mxfp4 returns them -> (rows, K)"""
-    _need(isinstance(op, (tuple, list)) and len(op) == 2, f"{what}: expected the pair that quant_mxfp4 returns")
+    if not isinstance(op, (tuple, list)) or len(op) != 2:
+        _refuse(f"{what}: expected the pair that quant_mxfp4 returns")
     codes, scales = op
-    _need(codes.dtype == torch.uint8 and codes.dim() == 2 and codes.is_contiguous() and codes.shape[1] > 0 and codes.shape[1] % 16 == 0,
-          f"{what}: codes must be contiguous uint8 [rows, K / 2], K a multiple of 32 (got {codes.dtype} {tuple(codes.shape)})")
-    rows, K = codes.shape[0], codes.shape[1] * 2
-    _need(scales.dtype == torch.uint8 and scales.is_contiguous() and tuple(scales.shape) == ((K + 255) // 256, rows, 8),
-          f"{what}: scales must be contiguous uint8 {((K + 255) // 256, rows, 8)} (got {scales.dtype} {tuple(scales.shape)})")
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_contiguous() or codes.shape[1] == 0 or codes.shape[1] % 16:
+        _refuse(f"{what}: codes must be contiguous uint8 [rows, K / 2], K a multiple of 32 (got {codes.dtype} {tuple(codes.shape)})")
+    rows, K = codes.shape
+    K *= 2
+    if scales.dtype != torch.uint8 or scales.shape != ((K + 255) // 256, rows, 8) or not scales.is_contiguous():
+        _refuse(f"{what}: scales must be contiguous uint8 {((K + 255) // 256, rows, 8)} (got {scales.dtype} {tuple(scales.shape)})")
     return rows, K
+
+
+def rmsnorm(x, w, *, res=None, fmt="same", h=None, rstd=None, eps=1e-6):
+    """Root-mean-square norm with the residual's addition (dist_op_rmsnorm): h = x + res, y = h / sqrt(mean h^2 + eps) * w over x [rows, C] (bf16 / fp32; w fp32).
+    fmt "same": y in x's type; "e4m3": bytes `q` and fp32 `scale` per row (what quant_rows_fp8 returns); "mxfp4": `codes` and `scales` (what quant_mxfp4 returns).
+    `h` is returned in x's type when `res` is given (or a buffer for it is: it may be x or res itself); `rstd` (fp32 [rows]) is filled when given, for rmsnorm_bwd.
+    Returns dict(y | q, scale | codes, scales [, h])."""
+    code = RMS_FMTS.get(fmt)
+    if code is None:
+        _refuse(f"fmt {fmt!r}: one of {sorted(RMS_FMTS)}")
+    dtype, shape = x.dtype, x.shape
+    dt = _dt(x)
+    if len(shape) != 2 or shape[1] == 0:
+        _refuse(f"x: expected [rows, C] with C > 0, got {tuple(shape)}")
+    rows, Cc = shape
+    ldx = _matrix(x, shape, "x", dtype)
+    _vector(w, Cc, "w")
+    if rstd is not None:
+        _vector(rstd, rows, "rstd")
+    ldres = _matrix(res, shape, "res", dtype) if res is not None else 0
+    dev = _device(x, w, res, h, rstd)
+    out = {}
+    if h is not None:
+        ldh = _matrix(h, shape, "h", dtype)
+        _apart(h, "h", x, res)
+    elif res is not None:
+        h, ldh = torch.empty(shape, dtype=dtype, device=x.device), Cc
+    if h is not None:
+        out["h"] = h
+    if code == L.RMS_SAME:
+        y, sc = torch.empty(shape, dtype=dtype, device=x.device), None
+        out["y"] = y
+    elif code == L.RMS_E4M3:
+        y, sc = torch.empty(shape, dtype=torch.uint8, device=x.device), torch.empty(rows, dtype=torch.float32, device=x.device)
+        out["q"], out["scale"] = y, sc
+    else:
+        y, sc = _mx_empty(rows, Cc, x.device)
+        out["codes"], out["scales"] = y, sc
+    a = L.RmsArgs(x.data_ptr(), res.data_ptr() if res is not None else None, h.data_ptr() if h is not None else None, w.data_ptr(), y.data_ptr(),
+                  sc.data_ptr() if sc is not None else None, rstd.data_ptr() if rstd is not None else None, rows, ldx, ldres, ldh if h is not None else 0, Cc, Cc, code, dt, eps)
+    _launch(dev, L.load().dist_op_rmsnorm, C.byref(a))
+    return out
+
+
+def rmsnorm_bwd(h, rstd, dy, w, *, dres=None, dh=None, dw=None):
+    """Backward of rmsnorm from its h and rstd (dist_op_rmsnorm_bwd); dy [rows, C] in bf16 or fp32, dres (h's type): the gradient that reaches h past the norm, added to dh.
+    dh: a buffer for the result (it may be dres, h or dy itself); dw (fp32 [C]) is ACCUMULATED into when given.  Returns (dh, dw).  The same bits every time."""
+    dt, dyt = _dt(h), _dt(dy)
+    dtype, shape = h.dtype, h.shape
+    if len(shape) != 2 or shape[1] == 0:
+        _refuse(f"h: expected [rows, C] with C > 0, got {tuple(shape)}")
+    rows, Cc = shape
+    ldh, lddy = _matrix(h, shape, "h", dtype), _matrix(dy, shape, "dy", dy.dtype)
+    _vector(w, Cc, "w")
+    _vector(rstd, rows, "rstd")
+    lddres = _matrix(dres, shape, "dres", dtype) if dres is not None else 0
+    dev = _device(h, rstd, dy, w, dres, dh, dw)
+    if dh is None:
+        dh, lddh = torch.empty(shape, dtype=dtype, device=h.device), Cc
+    else:
+        lddh = _matrix(dh, shape, "dh", dtype)
+        _apart(dh, "dh", h, dy, dres)
+    accumulate = int(dw is not None)
+    if dw is None:
+        dw = torch.empty(Cc, dtype=torch.float32, device=h.device)
+    else:
+        _vector(dw, Cc, "dw")
+    lib = L.load()
+    n = lib.dist_op_rmsnorm_bwd_scratch(rows, Cc)
+    scratch = torch.empty(n, dtype=torch.float32, device=h.device)
+    a = L.RmsBwdArgs(h.data_ptr(), rstd.data_ptr(), dy.data_ptr(), w.data_ptr(), dres.data_ptr() if dres is not None else None, dh.data_ptr(), dw.data_ptr(), scratch.data_ptr(),
+                     n, rows, ldh, lddy, lddres, lddh, Cc, dt, dyt, accumulate)
+    _launch(dev, lib.dist_op_rmsnorm_bwd, C.byref(a))
+    return dh, dw
 
 
 def quant_mxfp4(x, *, transpose=False):
     """x [rows, cols] (bf16 / fp32) in microscaled 4-bit floating point (dist_op_quant_mxfp4): (codes uint8 [rows, Kp / 2], scales uint8 [chunks, rows, 8]), blocks of 32 along
     the columns; transpose=True: of x^T, codes [cols, Kp / 2], blocks along x's rows.  Kp is the length of the blocked axis rounded up to 32 (zeros behind it)."""
-    lib = L.load()
     dt = _dt(x)
-    _need(x.dim() == 2, f"x: expected a matrix, got {tuple(x.shape)}")
+    if x.dim() != 2:
+        _refuse(f"x: expected a matrix, got {tuple(x.shape)}")
     rows, cols = x.shape
-    ld = _rows(x, rows, cols, "x")
+    ld = _matrix(x, x.shape, "x", x.dtype)
     n, K = (cols, rows) if transpose else (rows, cols)
-    _need(K > 0, "the quantised axis is empty")
-    with _on_device(x):
-        codes, scales = _mx_empty(n, K, x.device)
-        L.check(lib.dist_op_quant_mxfp4(x.data_ptr(), dt, rows, cols, ld, int(transpose), codes.data_ptr(), scales.data_ptr(), _stream()))
+    if K == 0:
+        _refuse("the quantised axis is empty")
+    dev = _device(x)
+    codes, scales = _mx_empty(n, K, x.device)
+    _launch(dev, L.load().dist_op_quant_mxfp4, x.data_ptr(), dt, rows, cols, ld, int(transpose), codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
 def dequant_mxfp4(codes, scales, dtype=torch.bfloat16):
     """the values (codes, scales) of quant_mxfp4 stand for, [rows, Kp] in `dtype` (bf16 / fp32; exact) (dist_op_dequant_mxfp4)"""
-    lib = L.load()
     rows, K = _mx_operand((codes, scales), "operand")
-    with _on_device(codes, scales):
-        y = torch.empty(rows, K, dtype=dtype, device=codes.device)
-        L.check(lib.dist_op_dequant_mxfp4(codes.data_ptr(), scales.data_ptr(), rows, K, y.data_ptr(), _dt(y), _stream()))
+    dev = _device(codes, scales)
+    y = torch.empty(rows, K, dtype=dtype, device=codes.device)
+    _launch(dev, L.load().dist_op_dequant_mxfp4, codes.data_ptr(), scales.data_ptr(), rows, K, y.data_ptr(), _dt(y))
     return y
 
 
@@ -726,44 +740,43 @@ def gemm_mxfp4(A, B, *, bias=None, res=None, out=None, out_dtype=torch.bfloat16)
     rmsnorm(fmt="mxfp4")), or (q uint8 [M, K], scale fp32 [M]) from rmsnorm(fmt="e4m3") / quant_rows_fp8.  bias fp32 [N]; res [M, N] in C's type (it may be `out` itself).
     C is bf16, or fp32 with an MXFP4 A.  The gradients are the same call: dA = gemm_mxfp4(quant_mxfp4(dC), quant_mxfp4(W, transpose=True)),
     dW = gemm_mxfp4(quant_mxfp4(dC, transpose=True), quant_mxfp4(X, transpose=True))."""
-    lib = L.load()
     N, K = _mx_operand(B, "B")
-    _need(N > 0, "B has no rows")
-    _need(isinstance(A, (tuple, list)) and len(A) == 2, "A: expected a pair (codes, scales) or (q, scale)")
-    a = L.GemmMxArgs()
+    if N == 0:
+        _refuse("B has no rows")
+    if not isinstance(A, (tuple, list)) or len(A) != 2:
+        _refuse("A: expected a pair (codes, scales) or (q, scale)")
     q, sc = A
     if sc.dtype == torch.float32:
-        _need(q.dim() == 2 and q.shape[1] == K, f"A: expected [M, {K}] e4m3 bytes, got {tuple(q.shape)}")
+        if q.dim() != 2 or q.shape[1] != K:
+            _refuse(f"A: expected [M, {K}] e4m3 bytes, got {tuple(q.shape)}")
         M = q.shape[0]
-        lda = _rows(q, M, K, "A", torch.uint8)
-        _need(lda % 16 == 0 and q.data_ptr() % 16 == 0, "A: rows of e4m3 bytes must start at multiples of 16 bytes")
+        lda = _matrix(q, q.shape, "A", torch.uint8)
+        if lda % 16 or q.data_ptr() % 16:
+            _refuse("A: rows of e4m3 bytes must start at multiples of 16 bytes")
         _vector(sc, M, "A's scale")
-        a.a_fmt, a.lda = L.MX_A_E4M3, lda
+        fmt = L.MX_A_E4M3
     else:
         M, Ka = _mx_operand(A, "A")
-        _need(Ka == K, f"A has {Ka} elements a row, B has {K}")
-        a.a_fmt = L.MX_A_MXFP4
-    with _on_device(B[0], B[1], q, sc, bias, res, out):
-        if out is None:
-            out = torch.empty(M, N, dtype=out_dtype, device=q.device)
-        elif M > 0:
-            _rows(out, M, N, "out")
-            for t in (q, B[0]):
-                _apart(out, t, "out", same_ok=False)
-        a.dtype = _dt(out)
-        _need(a.a_fmt == L.MX_A_MXFP4 or a.dtype == L.BF16, "a product with an e4m3 operand gives bf16")
-        a.ldc = _rows(out, M, N, "out")
-        if bias is not None:
-            _vector(bias, N, "bias")
-            a.bias = bias.data_ptr()
-        if res is not None:
-            a.res, a.ldres = res.data_ptr(), _rows(res, M, N, "res", out.dtype)
-            _apart(out, res, "out")
-        n = lib.dist_op_gemm_mxfp4_scratch(M, N, K, a.a_fmt)
-        if n > 0:
-            scratch = torch.empty(n, dtype=torch.float32, device=q.device)
-            a.scratch, a.scratch_elems = scratch.data_ptr(), n
-        a.A, a.a_scale, a.B, a.b_scale, a.C = q.data_ptr(), sc.data_ptr(), B[0].data_ptr(), B[1].data_ptr(), out.data_ptr()
-        a.M, a.N, a.K = M, N, K
-        L.check(lib.dist_op_gemm_mxfp4(C.byref(a), _stream()))
+        if Ka != K:
+            _refuse(f"A has {Ka} elements a row, B has {K}")
+        fmt, lda = L.MX_A_MXFP4, 0
+    dev = _device(q, sc, B[0], B[1], bias, res, out)
+    if out is None:
+        out, ldc = torch.empty(M, N, dtype=out_dtype, device=q.device), N
+    else:
+        ldc = _matrix(out, (M, N), "out", out.dtype)
+        _apart(out, "out", res)
+        _apart(out, "out", q, B[0], may_be=False)
+    dt = _dt(out)
+    if fmt == L.MX_A_E4M3 and dt != L.BF16:
+        _refuse("a product with an e4m3 operand gives bf16")
+    if bias is not None:
+        _vector(bias, N, "bias")
+    ldres = _matrix(res, (M, N), "res", out.dtype) if res is not None else 0
+    lib = L.load()
+    n = lib.dist_op_gemm_mxfp4_scratch(M, N, K, fmt)
+    scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None
+    a = L.GemmMxArgs(q.data_ptr(), sc.data_ptr(), B[0].data_ptr(), B[1].data_ptr(), bias.data_ptr() if bias is not None else None, res.data_ptr() if res is not None else None, out.data_ptr(),
+                     scratch.data_ptr() if n > 0 else None, M, lda, ldc, ldres, n, N, K, fmt, dt)
+    _launch(dev, lib.dist_op_gemm_mxfp4, C.byref(a))
     return out
