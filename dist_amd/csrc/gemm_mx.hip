@@ -3,15 +3,15 @@
 // One v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 x 16 outputs over 128 elements, the block scales applied by the instruction.  A lane holds for its row (lane & 15)
 // the 32 elements of block g = lane >> 4: 16 bytes of codes as they lie in memory.  An e4m3 operand has its 32 bytes in two runs of 16: elements 16 g .. and 64 + 16 g ..
 // (measured with random operands; the scale of lane group g still belongs to block g, here 1 for all).
-// The weight is the instruction's FIRST operand: the result has the outputs' n along the registers of a lane and m along the lanes, and with the weight's rows dealt to the
-// NT fragments as n = (i >> 2) * 4 NT + 4 j + (i & 3) (fragment j, its row i) a lane owns 4 NT consecutive outputs of one row of C: 16-byte stores, whole 128-byte lines
-// from four lanes at NT = 4, no exchange through LDS.
+// The weight is the instruction's FIRST operand: the result has the outputs' n along the registers of a lane and m along the lanes, so a lane owns consecutive outputs of
+// one row of C.
 #include <type_traits>
 #include "mx.h"
 
 namespace {
 
 typedef int v8i_t __attribute__((ext_vector_type(8)));
+typedef unsigned v4u_t __attribute__((ext_vector_type(4)));
 typedef int v4i_t __attribute__((ext_vector_type(4)));
 constexpr int NT_ = 256;
 
@@ -23,108 +23,88 @@ template <bool A8, int S> DEV void mma(const v8i_t& b, const v8i_t& a, f32x4& ac
     acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, acc, 4, A8 ? 0 : 4, S, bs, A8 ? 0 : S, as);
 }
 
-// 4 NT consecutive outputs of row m, from column n on
-template <bool A8, typename TO, int NT>
-DEV void store_row(const dist_gemm_mx_args& p, const f32x4 (&acc)[NT], long m, int n, bool vec) {
-    if (m >= p.M || n >= p.N) return;
-    float v[4 * NT];
-    const float as = A8 ? static_cast<const float*>(p.a_scale)[m] : 1.f;
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[4 * j + r] = A8 ? acc[j][r] * as : acc[j][r];
-    TO* C = static_cast<TO*>(p.C) + m * p.ldc + n;
-    const TO* R = p.res ? static_cast<const TO*>(p.res) + m * p.ldres + n : nullptr;
-    if (vec && n + 4 * NT <= p.N) {
-        if constexpr (NT % 2 == 0) {
-#pragma unroll
-            for (int j = 0; j < NT / 2; ++j) {
-                if (p.bias) { float b[8]; mx::load_v<8>(p.bias + n + 8 * j, b);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[8 * j + e] += b[e]; }
-                if (R) { float b[8]; mx::load_v<8>(R + 8 * j, b);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[8 * j + e] += b[e]; }
-                mx::store_v<8>(C + 8 * j, v + 8 * j);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                if (p.bias) { float b[4]; load4(p.bias + n + 4 * j, b);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[4 * j + e] += b[e]; }
-                if (R) { float b[4]; load4(R + 4 * j, b);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[4 * j + e] += b[e]; }
-                store4(C + 4 * j, v + 4 * j);
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 4 * NT; ++e)
-        if (n + e < p.N) C[e] = from_f<TO>(v[e] + (p.bias ? p.bias[n + e] : 0.f) + (R ? to_f(R[e]) : 0.f));
-}
-
-// Every wave a 16 MT x 16 NT tile of its own, fragments straight from global memory.
-template <bool A8, typename TO, int MT, int NT>
-__global__ __launch_bounds__(NT_) void gemm_mx_direct_kernel(const dist_gemm_mx_args p, const int vec, const int ntn) {
+// ---- few rows (one token, a handful of sequences): bound by the weight's bytes and by latency --------------------------------------------------------------------------
+// A workgroup owns 16 NT columns and all rows; its W waves share K, every wave's fragments come straight from global memory (a row's 128 elements are 64 bytes from four
+// lanes), and the partial sums meet in LDS, added in the waves' order.
+template <bool A8, typename TO, int MT, int NT, int W>
+__global__ __launch_bounds__(64 * W) void gemm_mx_few_kernel(const dist_gemm_mx_args p) {
+    constexpr int TILES = MT * NT;
+    __shared__ f32x4 part[W][TILES][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    const long m0 = ((long)(blockIdx.x / ntn) * 2 + (wave >> 1)) * (16 * MT);
-    const int n0 = ((int)(blockIdx.x % ntn) * 2 + (wave & 1)) * (16 * NT);
-    if (m0 >= p.M || n0 >= p.N) return;
+    const int n0 = blockIdx.x * (16 * NT);
     const unsigned char *A = static_cast<const unsigned char*>(p.A), *B = static_cast<const unsigned char*>(p.B);
     const unsigned char *SA = static_cast<const unsigned char*>(p.a_scale), *SB = static_cast<const unsigned char*>(p.b_scale);
     long am[MT], bn[NT];                                     // rows, clamped: what lies behind the last one is computed and not stored
 #pragma unroll
-    for (int t = 0; t < MT; ++t) am[t] = min(m0 + t * 16 + i, p.M - 1);
+    for (int t = 0; t < MT; ++t) am[t] = min((long)t * 16 + i, p.M - 1);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) bn[j] = min((long)n0 + (i >> 2) * (4 * NT) + 4 * j + (i & 3), (long)p.N - 1);
+    for (int j = 0; j < NT; ++j) bn[j] = min((long)n0 + j * 16 + i, (long)p.N - 1);
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const v4i_t zero = {0, 0, 0, 0};
-    for (int k0 = 0; k0 < p.K; k0 += mx::CHUNK) {
+#pragma unroll 2
+    for (int k = wave * 128; k < p.K; k += W * 128) {
+        const long chunk = k >> 8;
+        const int at = 2 * g + ((k >> 7) & 1);
+        const bool in = k + g * 32 < p.K;
+        v8i_t a[MT], b[NT];
         int as[MT], bs[NT];
-        const long chunk = k0 / mx::CHUNK;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) as[t] = A8 ? 127 : *reinterpret_cast<const unsigned short*>(SA + (chunk * p.M + am[t]) * 8 + 2 * g);
+        for (int j = 0; j < NT; ++j) {
+            b[j] = widen(in ? *reinterpret_cast<const v4i_t*>(B + bn[j] * (p.K / 2) + k / 2 + g * 16) : zero);
+            bs[j] = SB[(chunk * p.N + bn[j]) * 8 + at];
+        }
 #pragma unroll
-        for (int j = 0; j < NT; ++j) bs[j] = *reinterpret_cast<const unsigned short*>(SB + (chunk * p.N + bn[j]) * 8 + 2 * g);
-        auto step = [&](auto sc) {
-            constexpr int S = decltype(sc)::value;
-            const int k = k0 + S * 128;
-            if (k >= p.K) return;
-            v8i_t a[MT], b[NT];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) b[j] = widen(k + g * 32 < p.K ? *reinterpret_cast<const v4i_t*>(B + bn[j] * (p.K / 2) + k / 2 + g * 16) : zero);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                if constexpr (A8) {
-                    const unsigned char* q = A + am[t] * p.lda + k;
-                    a[t] = join(k + g * 16 < p.K ? *reinterpret_cast<const v4i_t*>(q + g * 16) : zero, k + 64 + g * 16 < p.K ? *reinterpret_cast<const v4i_t*>(q + 64 + g * 16) : zero);
-                } else a[t] = widen(k + g * 32 < p.K ? *reinterpret_cast<const v4i_t*>(A + am[t] * (p.K / 2) + k / 2 + g * 16) : zero);
+        for (int t = 0; t < MT; ++t) {
+            if constexpr (A8) {
+                const unsigned char* q = A + am[t] * p.lda + k;
+                a[t] = join(k + g * 16 < p.K ? *reinterpret_cast<const v4i_t*>(q + g * 16) : zero, k + 64 + g * 16 < p.K ? *reinterpret_cast<const v4i_t*>(q + 64 + g * 16) : zero);
+                as[t] = 127;
+            } else {
+                a[t] = widen(in ? *reinterpret_cast<const v4i_t*>(A + am[t] * (p.K / 2) + k / 2 + g * 16) : zero);
+                as[t] = SA[(chunk * p.M + am[t]) * 8 + at];
             }
+        }
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) mma<A8, S>(b[j], a[t], acc[t][j], bs[j], as[t]);
-        };
-        step(std::integral_constant<int, 0>{});
-        step(std::integral_constant<int, 1>{});
+            for (int j = 0; j < NT; ++j) mma<A8, 0>(b[j], a[t], acc[t][j], bs[j], as[t]);
     }
 #pragma unroll
-    for (int t = 0; t < MT; ++t) store_row<A8, TO, NT>(p, acc[t], m0 + t * 16 + i, n0 + g * (4 * NT), vec);
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) part[wave][t * NT + j][lane] = acc[t][j];
+    __syncthreads();
+    for (int e = threadIdx.x; e < TILES * 64; e += 64 * W) {                       // four neighbouring columns of a row
+        const int tile = e >> 6, l = e & 63;
+        const long m = (tile / NT) * 16 + (l & 15);
+        const int n = n0 + (tile % NT) * 16 + (l >> 4) * 4;
+        if (m >= p.M || n >= p.N) continue;
+        f32x4 s = part[0][tile][l];
+#pragma unroll
+        for (int w = 1; w < W; ++w) s += part[w][tile][l];
+        const float rs = A8 ? static_cast<const float*>(p.a_scale)[m] : 1.f;
+        TO* C = static_cast<TO*>(p.C) + m * p.ldc + n;
+        const TO* R = p.res ? static_cast<const TO*>(p.res) + m * p.ldres + n : nullptr;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (n + r < p.N) C[r] = from_f<TO>((A8 ? s[r] * rs : s[r]) + (p.bias ? p.bias[n + r] : 0.f) + (R ? to_f(R[r]) : 0.f));
+    }
 }
 
 // ---- tiles through LDS ------------------------------------------------------------------------------------------------------------------------------------------
 // WM x WN waves, each a 16 MT x 16 NT tile of outputs.  K advances by 128 elements a stage (one instruction deep): rows of 64 bytes of codes (e4m3: 128 bytes) go to LDS by
 // LDS-DMA into a ring of S stages, S - 1 of them in flight; one barrier per stage, behind a counted wait: when it opens, stage t has landed for every wave and stage
 // t - 1 is read by nobody, so its place receives stage t + S - 1.  Scale bytes follow per 256 elements into a ring of their own, with the stage that needs them first.
-// A 16-byte chunk c of row r lies at chunk c ^ f(r), applied where the DMA reads (its LDS side is lane-linear): the 16 rows a fragment read touches fall on
-// different banks.  Descriptors end behind the last row, and chunks behind K are sent past the end: all of these read as zeros.
+// A 16-byte chunk c of row r lies at chunk c ^ f(r), applied where the DMA reads (its LDS side is lane-linear).  Descriptors end behind the last row, and chunks behind K are
+// sent past the end: all of these read as zeros.
+// Measured (50432 x 2304 x 768, 4-bit operands, bf16 out): 95 us = 1.9 PF, of it 55 us when nothing is stored and 43 us when only the outputs are (5.4 TB/s): with six
+// stages a tile the workgroups of a CU stay in step, and the two add up.  Deep (16448 x 1024 x 4096, e4m3): 78 us = 1.8 PF, by the 41 GB/s a CU draws through its LDS-DMA.
+// Built and not faster: workgroups that stay and prefetch across tiles (88 - 91 and 97 us), fragments read half a stage ahead (no change), three or four stages in the ring,
+// all reads in front of the matrix instructions, raised priority around them (all within 3 %).
 typedef __attribute__((address_space(3))) void* lds_ptr;
 DEV void regs_pin(unsigned& v) { asm volatile("" : "+v"(v)); }
 template <int N> DEV void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
@@ -135,10 +115,10 @@ constexpr unsigned FAR_AWAY = 0x7ffffff0u;
 template <typename TO> DEV constexpr int frag_col(int j) { return sizeof(TO) == 2 ? (j >> 1) * 32 + (j & 1) * 4 : j * 16; }
 template <typename TO> DEV int lane_col(int i) { return sizeof(TO) == 2 ? (i >> 2) * 8 + (i & 3) : i; }
 
-template <bool A8> DEV int a_swz(int r) { return A8 ? (r >> 1) & 7 : ((r >> 2) & 1) | ((((r >> 1) ^ (r >> 3)) & 1) << 1); }
-template <typename TO> DEV int b_swz(int r) {
-    return sizeof(TO) == 2 ? ((r >> 3) & 1) | ((((r >> 1) ^ (r >> 4)) & 1) << 1) : a_swz<false>(r);
-}
+// (8 lanes read 128 bytes at a time: their 8 rows - consecutive ones of A, 0 ... 3 and 8 ... 11 of a 16-bit B - must fall on different 16-byte places.  ds_read_b128 then
+// moves 234 bytes a clock and CU; patterns that are free of conflicts over 16 lanes only reach 127.)
+template <bool A8> DEV int a_swz(int r) { return A8 ? (r >> 1) & 7 : (r >> 1) & 3; }
+template <typename TO> DEV int b_swz(int r) { return sizeof(TO) == 2 ? ((r >> 1) & 1) | ((r >> 2) & 2) : (r >> 1) & 3; }
 
 template <bool A8, typename TO, int WM, int WN, int MT, int NT, int S>
 struct Tile {
@@ -152,25 +132,27 @@ struct Tile {
     static_assert((NA + NB) % W == 0 && A_BYTES % 1024 == 0 && B_BYTES % 1024 == 0, "a stage is whole instructions for every wave");
 };
 
-template <bool A8, typename TO, int WM, int WN, int MT, int NT, int S, int OCC>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const dist_gemm_mx_args p, const int vec, const int ntm, const int ntn) {
+template <bool A8, bool RS, typename TO, int WM, int WN, int MT, int NT, int S, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const dist_gemm_mx_args p, const int fast, const int ntm, const int ntn, const int slice) {
     using T = Tile<A8, TO, WM, WN, MT, NT, S>;
     extern __shared__ char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const int wm = wave / WN, wn = wave % WN;
     // block -> tile: block b runs on XCD b % 8; every XCD takes a contiguous run of tiles, ordered in groups of 8 row tiles, so that the tiles an XCD works on at a time
     // share row and column panels in its L2
-    const int total = ntm * ntn, xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
-    const int t0 = xcd * each + min(xcd, more) + (int)(blockIdx.x >> 3);
+    const int total = ntm * ntn, part = blockIdx.x / total, block = blockIdx.x - part * total, xcd = block & 7, each = total >> 3, more = total & 7;
+    const int t0 = xcd * each + min(xcd, more) + (block >> 3);
     const int grp = t0 / (8 * ntn), in = t0 - grp * 8 * ntn, gm = min(8, ntm - grp * 8);
     const long m0 = (long)(grp * 8 + in % gm) * T::BM;
     const int n0 = (in / gm) * T::BN;
 
+    // elements k0 ... k0 + K of the long axis: all of them, or slice number `part` (then C is its fp32 partial result, without bias, residual and row scales)
+    const int k0 = part * slice, K = min(slice, p.K - k0), chunk0 = k0 >> 8;
     const long pitch_a = A8 ? p.lda : p.K / 2, pitch_b = p.K / 2;
-    const int mrows = (int)min((long)T::BM, p.M - m0), nrows = min(T::BN, p.N - n0);
-    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.A) + m0 * pitch_a), 0, (int)(mrows * pitch_a), 0x00020000);
-    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.B) + n0 * pitch_b), 0, (int)(nrows * pitch_b), 0x00020000);
-    const int nk = (p.K + 127) / 128, tail = p.K - (nk - 1) * 128;                 // elements of the last stage
+    const int mrows = (int)min((long)T::BM, p.M - m0), nrows = min(T::BN, p.N - n0), ka = A8 ? k0 : k0 / 2;
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.A) + m0 * pitch_a + ka), 0, (int)(mrows * pitch_a - ka), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.B) + n0 * pitch_b + k0 / 2), 0, (int)(nrows * pitch_b - k0 / 2), 0x00020000);
+    const int nk = (K + 127) / 128, tail = K - (nk - 1) * 128;                     // stages; elements of the last one
 
     // this wave's kilobytes of a stage: which operand, and the lane's offset in it
     unsigned voff[T::PER];
@@ -215,11 +197,11 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const d
         const int k = min(wave * T::PERS + q, T::NS - 1);
         sdst[q] = S * T::STAGE + k * 1024;
         if (k < T::SA_BYTES / 1024) {
-            ssrc[q] = static_cast<const char*>(p.a_scale) + m0 * 8 + k * 1024;
+            ssrc[q] = static_cast<const char*>(p.a_scale) + ((long)chunk0 * p.M + m0) * 8 + k * 1024;
             sstep[q] = p.M * 8;
             sleft[q] = max(mrows * 8 - k * 1024, 0);
         } else {
-            ssrc[q] = static_cast<const char*>(p.b_scale) + (long)n0 * 8 + (k * 1024 - T::SA_BYTES);
+            ssrc[q] = static_cast<const char*>(p.b_scale) + ((long)chunk0 * p.N + n0) * 8 + (k * 1024 - T::SA_BYTES);
             sstep[q] = (long)p.N * 8;
             sleft[q] = max(nrows * 8 - (k * 1024 - T::SA_BYTES), 0);
         }
@@ -296,77 +278,180 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const d
     const long mw = m0 + wm * MT * 16 + i;
     float rs[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) rs[t] = A8 && mw + t * 16 < p.M ? static_cast<const float*>(p.a_scale)[mw + t * 16] : 1.f;
-    constexpr int G = sizeof(TO) == 2 ? 2 : 1, V = 4 * G;                          // fragments and outputs of one 16-byte store
+    for (int t = 0; t < MT; ++t) rs[t] = A8 && RS && mw + t * 16 < p.M ? static_cast<const float*>(p.a_scale)[mw + t * 16] : 1.f;
+    // 16-byte stores through a descriptor that ends behind the last row; columns behind N are sent past it.  Lanes i and i ^ 8 exchange, so that a store writes 8 rows of
+    // 128 bytes and not 16 of 64, past the caches' keeping: a 232 MB output takes 43 us this way and 64 us in half lines kept in the L2
+    constexpr int U = sizeof(TO) == 2 ? 2 : 1, ES = sizeof(TO);                    // fragments of one 16-byte store
+    const int rowl = wm * MT * 16 + i, coll = wn * NT * 16 + g * (4 * U);
+    TO* const C = static_cast<TO*>(p.C) + part * (p.M * p.ldc);                    // (slices lie one behind the other)
+    if (fast) {
+        const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(C) + (m0 * p.ldc + n0) * ES, 0, (int)((mrows * p.ldc - n0) * ES), 0x00020000);
+        const __amdgpu_buffer_rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.res)) + (m0 * p.ldres + n0) * ES, 0, p.res ? (int)((mrows * p.ldres - n0) * ES) : 0, 0x00020000);
+        const bool up = (i & 8) != 0;
+        const int rowx = rowl - (up ? 8 : 0);
 #pragma unroll
-    for (int j = 0; j < NT; j += G) {
-        const int n = n0 + wn * NT * 16 + frag_col<TO>(j) + g * V;
-        if (n >= p.N) continue;
-        const bool whole = vec && n + V <= p.N;
-        float bias[V];
+        for (int j = 0; j < NT; j += 2 * U) {
+            const int col = coll + frag_col<TO>(j) + (up ? frag_col<TO>(U) : 0);
+            const bool in = n0 + col < p.N;
+            v4u_t q[MT][2];
+            if (p.res) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) bias[e] = 0.f;
-        if (p.bias) {
-            if (whole) {
-                if constexpr (V == 8) mx::load_v<8>(p.bias + n, bias);
-                else load4(p.bias + n, bias);
-            } else {
+                for (int t = 0; t < MT; ++t) {
+                    const unsigned o = (unsigned)(((rowx + t * 16) * p.ldres + col) * ES);
+                    q[t][0] = __builtin_amdgcn_raw_buffer_load_b128(rr, in ? o : FAR_AWAY, 0, 0);
+                    q[t][1] = __builtin_amdgcn_raw_buffer_load_b128(rr, in ? o + (unsigned)(8 * p.ldres * ES) : FAR_AWAY, 0, 0);
+                }
+            }
+            float bias[2][4 * U];
 #pragma unroll
-                for (int e = 0; e < V; ++e) bias[e] = n + e < p.N ? p.bias[n + e] : 0.f;
+            for (int h = 0; h < 2; ++h) {
+                const int n = n0 + coll + frag_col<TO>(j + h * U);
+#pragma unroll
+                for (int e = 0; e < 4 * U; ++e) bias[h][e] = 0.f;
+                if (p.bias && n < p.N) {
+                    if constexpr (U == 2) mx::load_v<8>(p.bias + n, bias[h]);
+                    else load4(p.bias + n, bias[h]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                float own[2][4 * U];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4 * U; ++e) own[h][e] = (A8 ? acc[t][j + h * U + e / 4][e % 4] * rs[t] : acc[t][j + h * U + e / 4][e % 4]) + bias[h][e];
+                if (p.res) {                                                       // in fp32: exchange, add, round
+#pragma unroll
+                    for (int e = 0; e < 4 * U; ++e) {
+                        const float got = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(up ? own[0][e] : own[1][e]), 0x128 /* row_ror:8 */, 0xf, 0xf, true));
+                        if (up) own[0][e] = got; else own[1][e] = got;
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if constexpr (U == 2) {
+                            const bf16x8 f = __builtin_bit_cast(bf16x8, q[t][h]);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) own[h][e] += (float)f[e];
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) own[h][e] += __uint_as_float(q[t][h][e]);
+                        }
+                    }
+                }
+                v4u_t out[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if constexpr (U == 2) {
+                        Frag<bf16_t> f;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) frag_set(f, e, own[h][e]);
+                        out[h] = __builtin_bit_cast(v4u_t, f.v);
+                    } else out[h] = v4u_t{__float_as_uint(own[h][0]), __float_as_uint(own[h][1]), __float_as_uint(own[h][2]), __float_as_uint(own[h][3])};
+                }
+                if (!p.res) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const unsigned got = __builtin_amdgcn_update_dpp(0, (int)(up ? out[0][e] : out[1][e]), 0x128, 0xf, 0xf, true);
+                        if (up) out[0][e] = got; else out[1][e] = got;
+                    }
+                }
+                const unsigned o = (unsigned)(((rowx + t * 16) * p.ldc + col) * ES);
+                __builtin_amdgcn_raw_buffer_store_b128(out[0], rc, in ? o : FAR_AWAY, 0, 2);
+                __builtin_amdgcn_raw_buffer_store_b128(out[1], rc, in ? o + (unsigned)(8 * p.ldc * ES) : FAR_AWAY, 0, 2);
             }
         }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             const long m = mw + t * 16;
-            if (m >= p.M) continue;
-            TO* C = static_cast<TO*>(p.C) + m * p.ldc + n;
-            const TO* R = p.res ? static_cast<const TO*>(p.res) + m * p.ldres + n : nullptr;
-            float v[V];
+            const int c = wn * NT * 16 + frag_col<TO>(j & ~(U - 1)) + g * (4 * U) + (j & (U - 1)) * 4;
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = (A8 ? acc[t][j + e / 4][e % 4] * rs[t] : acc[t][j + e / 4][e % 4]) + bias[e];
-            if (whole) {
-                float r[V];
-                if constexpr (V == 8) {
-                    if (R) { mx::load_v<8>(R, r);
-#pragma unroll
-                        for (int e = 0; e < V; ++e) v[e] += r[e]; }
-                    mx::store_v<8>(C, v);
-                } else {
-                    if (R) { load4(R, r);
-#pragma unroll
-                        for (int e = 0; e < V; ++e) v[e] += r[e]; }
-                    store4(C, v);
+            for (int e = 0; e < 4; ++e)
+                if (m < p.M && n0 + c + e < p.N) {
+                    const float v = (A8 ? acc[t][j][e] * rs[t] : acc[t][j][e]) + (p.bias ? p.bias[n0 + c + e] : 0.f);
+                    C[m * p.ldc + n0 + c + e] = from_f<TO>(v + (p.res ? to_f(static_cast<const TO*>(p.res)[m * p.ldres + n0 + c + e]) : 0.f));
                 }
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (n + e < p.N) C[e] = from_f<TO>(v[e] + (R ? to_f(R[e]) : 0.f));
-            }
         }
-    }
 }
 
-template <bool A8, typename TO, int WM, int WN, int MT, int NT, int S, int OCC> int launch_tile(const dist_gemm_mx_args& p, int vec, hipStream_t s) {
+// C = bias + res + a_scale * sum of the slices, in their order
+template <bool A8, typename TO>
+__global__ __launch_bounds__(NT_) void gemm_mx_join_kernel(const dist_gemm_mx_args p, const float* __restrict__ part, const int parts) {
+    const long e = (long)blockIdx.x * NT_ + threadIdx.x, size = p.M * p.N;
+    if (e >= size) return;
+    const long m = e / p.N;
+    const int n = (int)(e - m * p.N);
+    float s = part[e];
+    for (int k = 1; k < parts; ++k) s += part[k * size + e];
+    if (A8) s *= static_cast<const float*>(p.a_scale)[m];
+    static_cast<TO*>(p.C)[m * p.ldc + n] = from_f<TO>(s + (p.bias ? p.bias[n] : 0.f) + (p.res ? to_f(static_cast<const TO*>(p.res)[m * p.ldres + n]) : 0.f));
+}
+
+template <bool A8, bool RS, typename TO, int WM, int WN, int MT, int NT, int S, int OCC> int launch_tile(const dist_gemm_mx_args& p, int slice, hipStream_t s) {
     using T = Tile<A8, TO, WM, WN, MT, NT, S>;
-    const long ntm = (p.M + T::BM - 1) / T::BM, ntn = (p.N + T::BN - 1) / T::BN;
-    if (ntm * ntn > 0x3fffffff) return DIST_ERR_ARG;
-    const auto k = gemm_mx_tile_kernel<A8, TO, WM, WN, MT, NT, S, OCC>;
+    const long ntm = (p.M + T::BM - 1) / T::BM, ntn = (p.N + T::BN - 1) / T::BN, parts = (p.K + slice - 1) / slice;
+    if (ntm * ntn * parts > 0x3fffffff) return DIST_ERR_ARG;
+    const auto k = gemm_mx_tile_kernel<A8, RS, TO, WM, WN, MT, NT, S, OCC>;
     static DistSmemOnce st;
     RUN_(dist_max_smem(st, reinterpret_cast<const void*>(k), T::LDS));
-    hipLaunchKernelGGL(k, dim3((unsigned)(ntm * ntn)), dim3(64 * T::W), T::LDS, s, p, vec, (int)ntm, (int)ntn);
+    constexpr size_t ES = sizeof(TO);
+    const bool fast = p.N % (16 / ES) == 0 && (uintptr_t)p.C % 16 == 0 && p.ldc * ES % 16 == 0 && p.ldc <= 1 << 20 && (!p.bias || (uintptr_t)p.bias % 16 == 0) &&
+                      (!p.res || ((uintptr_t)p.res % 16 == 0 && p.ldres * ES % 16 == 0 && p.ldres <= 1 << 20));
+    hipLaunchKernelGGL(k, dim3((unsigned)(ntm * ntn * parts)), dim3(64 * T::W), T::LDS, s, p, (int)fast, (int)ntm, (int)ntn, slice);
+    HIP_CHECK_RET(hipGetLastError());
+    return DIST_OK;
+}
+
+enum { FEW = 0, SMALL = 1, SQUARE = 2, WIDE = 3 };
+struct Plan { int kind, slice; };
+constexpr int LIMIT = 1 << 22;                               // bytes of a row (128 rows of a tile lie within 32-bit offsets)
+
+// Which kernel (times in us, inputs out of the caches, bias; kernels of this file beside each other):
+//   FEW     M <= 64: the tiles' ring has a long way to the first result.  N = K = 4096: 64 rows 9.1 against 10.9 in 64 x 64 tiles, 16 rows 4.8
+//   SMALL   64 x 64, where 128 x 128 would leave CUs without work (under 200 tiles): 788 x 2304 x 768 5.4 against 5.9; 2048 x 2048 x 1024 (256 tiles) 8.4 against 7.0 the other way.
+//           The long axis is cut where even these do not fill the 256 CUs, in slices of at least 2048 (shorter ones cost more in the joining pass than they gain:
+//           200 x 520 x 2048 7.1 whole, 7.7 in two)
+//   SQUARE  128 x 128, three workgroups a CU (768 places);  WIDE 128 x 256, two a CU (512 places), 4-bit operands only: a tile takes 1.5 times as long and does twice the work,
+//           so it is worth its places when its rounds are few enough: 4096^3 43 against 55, 6400 x 2304 x 768 13.4 against 15.6, but 16448 x 1024 x 4096 (516 tiles) 68 against 62
+Plan plan(int64_t M, int N, int K, int a_fmt) {
+    const int64_t t64 = (M + 63) / 64 * ((N + 63) / 64), t128 = (M + 127) / 128 * ((N + 127) / 128), t256 = (M + 127) / 128 * ((N + 255) / 256);
+    if (M <= 64) return Plan{FEW, K};
+    if (t128 >= 200)
+        return Plan{a_fmt == DIST_MX_A_MXFP4 && 3 * ((t256 + 511) / 512) <= 2 * ((t128 + 767) / 768) ? WIDE : SQUARE, K};
+    int parts = 1;
+    while (t64 * parts < 256 && K / (2 * parts) >= 2048) parts *= 2;
+    return Plan{SMALL, parts == 1 ? K : (K / parts + 255) / 256 * 256};
+}
+
+template <bool A8, typename TO, int MT, int NT, int W> int launch_few(const dist_gemm_mx_args& p, hipStream_t s) {
+    hipLaunchKernelGGL((gemm_mx_few_kernel<A8, TO, MT, NT, W>), dim3((unsigned)((p.N + 16 * NT - 1) / (16 * NT))), dim3(64 * W), 0, s, p);
     HIP_CHECK_RET(hipGetLastError());
     return DIST_OK;
 }
 
 template <bool A8, typename TO> int launch(const dist_gemm_mx_args& p, hipStream_t s) {
-    const size_t es = sizeof(TO);
-    const int vec = (uintptr_t)p.C % 16 == 0 && p.ldc * es % 16 == 0 && (!p.res || ((uintptr_t)p.res % 16 == 0 && p.ldres * es % 16 == 0)) && (!p.bias || (uintptr_t)p.bias % 16 == 0);
-    if (p.M > 64 && p.K <= 1 << 22 && p.lda <= 1 << 22) {
-        return launch_tile<A8, TO, 2, 2, 4, 4, 3, 2>(p, vec, s);
+    Plan w = plan(p.M, p.N, p.K, p.a_fmt);
+    if (w.kind == FEW) {
+        if (p.M <= 16) return launch_few<A8, TO, 1, 1, 8>(p, s);
+        if (p.M <= 32) return launch_few<A8, TO, 2, 1, 8>(p, s);
+        return launch_few<A8, TO, 4, 1, 8>(p, s);
     }
-    const long ntm = (p.M + 127) / 128, ntn = (p.N + 127) / 128;
-    if (ntm * ntn > 0x7fffffff) return DIST_ERR_ARG;
-    hipLaunchKernelGGL((gemm_mx_direct_kernel<A8, TO, 4, 4>), dim3((unsigned)(ntm * ntn)), dim3(NT_), 0, s, p, vec, (int)ntn);
+    if constexpr (!A8) {
+        if (w.kind == WIDE) return launch_tile<A8, true, TO, 2, 2, 4, 8, 2, 2>(p, p.K, s);
+    }
+    if (w.kind == SQUARE) return launch_tile<A8, true, TO, 2, 2, 4, 4, 2, 3>(p, p.K, s);
+    if (w.slice >= p.K) return launch_tile<A8, true, TO, 4, 1, 1, 4, 4, 4>(p, p.K, s);
+    dist_gemm_mx_args q = p;
+    q.C = p.scratch;
+    q.ldc = p.N;
+    q.bias = nullptr;
+    q.res = nullptr;
+    RUN_((launch_tile<A8, false, float, 4, 1, 1, 4, 4, 4>(q, w.slice, s)));
+    const long blocks = (p.M * p.N + NT_ - 1) / NT_;
+    hipLaunchKernelGGL((gemm_mx_join_kernel<A8, TO>), dim3((unsigned)blocks), dim3(NT_), 0, s, p, p.scratch, (p.K + w.slice - 1) / w.slice);
     HIP_CHECK_RET(hipGetLastError());
     return DIST_OK;
 }
@@ -375,7 +460,9 @@ template <bool A8, typename TO> int launch(const dist_gemm_mx_args& p, hipStream
 
 extern "C" int64_t dist_op_gemm_mxfp4_scratch(int64_t M, int N, int K, int a_fmt) {
     if (M < 0 || N <= 0 || K <= 0 || K % 32 || (a_fmt != DIST_MX_A_MXFP4 && a_fmt != DIST_MX_A_E4M3)) return -1;
-    return 0;
+    const Plan w = plan(M, N, K, a_fmt);
+    const int64_t parts = (K + w.slice - 1) / w.slice;
+    return parts > 1 ? parts * M * N : 0;
 }
 
 extern "C" int dist_op_gemm_mxfp4(const dist_gemm_mx_args* a, void* stream) {
@@ -383,14 +470,15 @@ extern "C" int dist_op_gemm_mxfp4(const dist_gemm_mx_args* a, void* stream) {
     const dist_gemm_mx_args p = *a;
     if (p.a_fmt != DIST_MX_A_MXFP4 && p.a_fmt != DIST_MX_A_E4M3) return DIST_ERR_ARG;
     if ((p.dtype != DIST_BF16 && p.dtype != DIST_F32) || (p.a_fmt == DIST_MX_A_E4M3 && p.dtype != DIST_BF16)) return DIST_ERR_ARG;
-    if (p.M < 0 || p.N <= 0 || p.K <= 0 || p.K % 32 || p.K > (1 << 30)) return DIST_ERR_ARG;
+    if (p.M < 0 || p.N <= 0 || p.K <= 0 || p.K % 32 || p.K > LIMIT) return DIST_ERR_ARG;
     if (p.M == 0) return DIST_OK;
     const uintptr_t es = p.dtype == DIST_BF16 ? 2 : 4;
     if (!p.A || !p.a_scale || !p.B || !p.b_scale || !p.C || p.ldc < p.N || (p.res && p.ldres < p.N)) return DIST_ERR_ARG;
     if ((uintptr_t)p.A % 16 || (uintptr_t)p.B % 16 || (uintptr_t)p.b_scale % 8 || (uintptr_t)p.a_scale % (p.a_fmt == DIST_MX_A_E4M3 ? 4 : 8)) return DIST_ERR_ARG;
-    if (p.a_fmt == DIST_MX_A_E4M3 && (p.lda < p.K || p.lda % 16)) return DIST_ERR_ARG;
+    if (p.a_fmt == DIST_MX_A_E4M3 && (p.lda < p.K || p.lda % 16 || p.lda > LIMIT)) return DIST_ERR_ARG;
     if ((uintptr_t)p.C % es || (uintptr_t)p.res % es || (uintptr_t)p.bias % 4) return DIST_ERR_ARG;
-    if (p.scratch_elems < dist_op_gemm_mxfp4_scratch(p.M, p.N, p.K, p.a_fmt)) return DIST_ERR_WORKSPACE;
+    const int64_t need = dist_op_gemm_mxfp4_scratch(p.M, p.N, p.K, p.a_fmt);
+    if (need > 0 && (p.scratch_elems < need || !p.scratch || (uintptr_t)p.scratch % 16)) return DIST_ERR_WORKSPACE;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (p.a_fmt == DIST_MX_A_E4M3) return launch<true, bf16_t>(p, s);
     return p.dtype == DIST_BF16 ? launch<false, bf16_t>(p, s) : launch<false, float>(p, s);
