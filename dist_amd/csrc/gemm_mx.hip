@@ -309,7 +309,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const d
 #pragma unroll
                 for (int e = 0; e < 4 * U; ++e) bias[h][e] = 0.f;
                 if (p.bias && n < p.N) {
-                    if constexpr (U == 2) mx::load_v<8>(p.bias + n, bias[h]);
+                    if constexpr (U == 2) mx::load_v8(p.bias + n, bias[h]);
                     else load4(p.bias + n, bias[h]);
                 }
             }

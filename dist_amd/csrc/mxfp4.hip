@@ -7,8 +7,7 @@ namespace {
 constexpr int NT = 256;
 
 // Along the rows.  32 lanes own a chunk of 256 elements of one row, 8 consecutive elements a lane: a block is four neighbouring lanes, its maximum two shuffles.
-// V = 1: any alignment and any tail, elements read one by one (a lane's loads past K give zeros).
-template <typename T, int V>
+template <typename T, bool AL>
 __global__ __launch_bounds__(NT) void quant_rows_kernel(const T* __restrict__ x, const long rows, const long K, const long ld, const int Kp, const int chunks,
                                                         unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
     const long item = (long)blockIdx.x * (NT / 32) + (threadIdx.x >> 5);
@@ -18,16 +17,7 @@ __global__ __launch_bounds__(NT) void quant_rows_kernel(const T* __restrict__ x,
     if (row >= rows) return;                                 // (a whole half-wave: the shuffles below stay inside it)
     const long c0 = (long)chunk * mx::CHUNK + lane * 8;
     float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    const T* xr = x + row * ld;
-    if constexpr (V == 8) {
-        if (c0 < K) mx::load_v<8>(xr + c0, v);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (c0 + e < K) v[e] = to_f(xr[c0 + e]);
-    }
+    mx::load8<AL>(x + row * ld + c0, K - c0, v);
     unsigned a = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) a = max(a, mx::abs_bits(v[e]));
@@ -38,29 +28,54 @@ __global__ __launch_bounds__(NT) void quant_rows_kernel(const T* __restrict__ x,
     if ((lane & 3) == 0) scales[mx::scale_at(row, rows, chunk * 8 + (lane >> 2))] = (unsigned char)(c0 < Kp ? byte : 0);
 }
 
-// Along the columns: output row c holds the elements x[:, c].  A wave owns one block (32 rows of x) of 64 columns: every load of a row is 64 neighbouring elements,
-// a lane ends with the 32 elements of its block and needs no exchange.
-template <typename T>
-__global__ __launch_bounds__(NT) void quant_cols_kernel(const T* __restrict__ x, const long R, const int C, const long ld, const long Kp, const long nblk, const int ctiles,
-                                                        unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
-    const long item = (long)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
-    const long ct = item / nblk, b = item - ct * nblk;
-    const int c = (int)ct * 64 + (threadIdx.x & 63);
-    if (ct >= ctiles || c >= C) return;
-    const long r0 = b * mx::BLOCK;
-    float v[32];
+// Along the columns: output row c holds the elements x[:, c].  A workgroup takes 256 rows of x (a chunk) and 64 VC columns, a wave one block of 32 rows: every load of a row is
+// 64 VC neighbouring elements, a lane ends with the 32 elements of its VC blocks and needs no exchange.  Codes and scales go through LDS, so that a column's 128
+// bytes of codes and the columns' 8 bytes of scales are written as whole lines.
+template <typename T, int VC>
+__global__ __launch_bounds__(512) void quant_cols_kernel(const T* __restrict__ x, const long R, const int C, const long ld, const long Kp, const int ctiles,
+                                                         unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
+    __shared__ uint4 lc[64 * VC][9];                          // (a 16-byte pad: the waves' columns fall on different banks)
+    __shared__ unsigned char ls[64 * VC][8];
+    typedef T vec_t __attribute__((ext_vector_type(VC)));
+    const int chunk = blockIdx.x / ctiles, lane = threadIdx.x & 63, b = threadIdx.x >> 6, ct0 = (blockIdx.x - chunk * ctiles) * 64 * VC, c = ct0 + lane * VC;
+    const long r0 = (long)chunk * mx::CHUNK + b * mx::BLOCK;
+    float v[VC][32];
+    if (c < C) {
+        const T* src = x + r0 * ld + c;
+        if (r0 + 32 <= R) {
+            vec_t w[32];
 #pragma unroll
-    for (int e = 0; e < 32; ++e) v[e] = r0 + e < R ? to_f(x[(r0 + e) * ld + c]) : 0.f;
-    unsigned a = 0;
+            for (int e = 0; e < 32; ++e) w[e] = *reinterpret_cast<const vec_t*>(src + e * ld);
 #pragma unroll
-    for (int e = 0; e < 32; ++e) a = max(a, mx::abs_bits(v[e]));
-    const int byte = mx::scale_byte(a);
-    if (r0 < Kp) {
-        uint4 w;
-        w.x = mx::pack8(v, byte); w.y = mx::pack8(v + 8, byte); w.z = mx::pack8(v + 16, byte); w.w = mx::pack8(v + 24, byte);
-        *reinterpret_cast<uint4*>(codes + (long)c * (Kp / 2) + r0 / 2) = w;
+            for (int e = 0; e < 32; ++e)
+#pragma unroll
+                for (int k = 0; k < VC; ++k) v[k][e] = to_f((T)w[e][k]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+#pragma unroll
+                for (int k = 0; k < VC; ++k) v[k][e] = r0 + e < R ? to_f(src[e * ld + k]) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < VC; ++k) {
+            unsigned a = 0;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) a = max(a, mx::abs_bits(v[k][e]));
+            const int byte = mx::scale_byte(a);
+            uint4 w;
+            w.x = mx::pack8(v[k], byte); w.y = mx::pack8(v[k] + 8, byte); w.z = mx::pack8(v[k] + 16, byte); w.w = mx::pack8(v[k] + 24, byte);
+            lc[lane * VC + k][b] = w;
+            ls[lane * VC + k][2 * (b & 3) + (b >> 2)] = (unsigned char)(r0 < Kp ? byte : 0);
+        }
     }
-    scales[mx::scale_at(c, C, (int)b)] = (unsigned char)(r0 < Kp ? byte : 0);
+    __syncthreads();
+    for (int q = threadIdx.x; q < 64 * VC * 8; q += 512) {
+        const int col = q >> 3, blk = q & 7;
+        const long k = (long)chunk * mx::CHUNK + blk * mx::BLOCK;
+        if (ct0 + col < C && k < Kp) *reinterpret_cast<uint4*>(codes + (ct0 + col) * (Kp / 2) + k / 2) = lc[col][blk];
+    }
+    if (threadIdx.x < 64 * VC && ct0 + (int)threadIdx.x < C)
+        *reinterpret_cast<uint2*>(scales + ((long)chunk * C + ct0 + threadIdx.x) * 8) = *reinterpret_cast<const uint2*>(ls[threadIdx.x]);
 }
 
 template <typename T>
@@ -73,7 +88,7 @@ __global__ __launch_bounds__(NT) void dequant_kernel(const unsigned char* __rest
     if (row >= rows) return;
     float v[8];
     mx::unpack8(reinterpret_cast<const unsigned*>(codes)[i], scales[mx::scale_at(row, rows, v8 / 4)], v);
-    mx::store_v<8>(y + i * 8, v);
+    mx::store8<true>(y + i * 8, 8, v);
 }
 
 }  // namespace
@@ -87,23 +102,24 @@ extern "C" int dist_op_quant_mxfp4(const void* x, int dtype, int64_t rows, int64
     const int64_t out_rows = transpose ? cols : rows, K = transpose ? rows : cols;
     if (K <= 0 || K > (1l << 30) || out_rows > (1l << 30)) return DIST_ERR_ARG;
     if (out_rows == 0) return DIST_OK;
-    if (!x || !codes || !scales || (uintptr_t)codes % 16 || (uintptr_t)x % (dtype == DIST_BF16 ? 2 : 4)) return DIST_ERR_ARG;
+    if (!x || !codes || !scales || (uintptr_t)codes % 16 || (uintptr_t)scales % 8 || (uintptr_t)x % (dtype == DIST_BF16 ? 2 : 4)) return DIST_ERR_ARG;
     hipStream_t s = static_cast<hipStream_t>(stream);
     unsigned char *q = static_cast<unsigned char*>(codes), *sc = static_cast<unsigned char*>(scales);
     const int64_t Kp = (K + 31) / 32 * 32, chunks = (K + mx::CHUNK - 1) / mx::CHUNK;
     if (!transpose) {
         const int64_t blocks = (rows * chunks + NT / 32 - 1) / (NT / 32);
         if (blocks > 0x7fffffff) return DIST_ERR_ARG;
-        const bool vec = cols % 8 == 0 && ld % 8 == 0 && (uintptr_t)x % 16 == 0;
-#define DIST_QR(T, V) hipLaunchKernelGGL((quant_rows_kernel<T, V>), dim3((unsigned)blocks), dim3(NT), 0, s, static_cast<const T*>(x), (long)rows, (long)K, (long)ld, (int)Kp, (int)chunks, q, sc)
-        if (dtype == DIST_BF16) { if (vec) DIST_QR(bf16_t, 8); else DIST_QR(bf16_t, 1); }
-        else { if (vec) DIST_QR(float, 8); else DIST_QR(float, 1); }
+        const bool al = cols % 8 == 0 && ld % 8 == 0 && (uintptr_t)x % 16 == 0;
+#define DIST_QR(T, AL) hipLaunchKernelGGL((quant_rows_kernel<T, AL>), dim3((unsigned)blocks), dim3(NT), 0, s, static_cast<const T*>(x), (long)rows, (long)K, (long)ld, (int)Kp, (int)chunks, q, sc)
+        if (dtype == DIST_BF16) { if (al) DIST_QR(bf16_t, true); else DIST_QR(bf16_t, false); }
+        else { if (al) DIST_QR(float, true); else DIST_QR(float, false); }
 #undef DIST_QR
     } else {
-        const int64_t nblk = chunks * 8, ctiles = (cols + 63) / 64, blocks = (ctiles * nblk + NT / 64 - 1) / (NT / 64);
+        const bool two = dtype == DIST_BF16 && cols % 2 == 0 && ld % 2 == 0 && (uintptr_t)x % 4 == 0;        // two bf16 columns a lane
+        const int64_t ctiles = two ? (cols + 127) / 128 : (cols + 63) / 64, blocks = ctiles * chunks;
         if (blocks > 0x7fffffff) return DIST_ERR_ARG;
-#define DIST_QC(T) hipLaunchKernelGGL((quant_cols_kernel<T>), dim3((unsigned)blocks), dim3(NT), 0, s, static_cast<const T*>(x), (long)rows, (int)cols, (long)ld, (long)Kp, (long)nblk, (int)ctiles, q, sc)
-        if (dtype == DIST_BF16) DIST_QC(bf16_t); else DIST_QC(float);
+#define DIST_QC(T, VC) hipLaunchKernelGGL((quant_cols_kernel<T, VC>), dim3((unsigned)blocks), dim3(512), 0, s, static_cast<const T*>(x), (long)rows, (int)cols, (long)ld, (long)Kp, (int)ctiles, q, sc)
+        if (two) DIST_QC(bf16_t, 2); else if (dtype == DIST_BF16) DIST_QC(bf16_t, 1); else DIST_QC(float, 1);
 #undef DIST_QC
     }
     HIP_CHECK_RET(hipGetLastError());

@@ -35,44 +35,44 @@ DEV float e4m3_factor(float a, float& scale) {
     return a > 0.f ? 448.f / b : 1.f;
 }
 
-// one group of V values of a row -> the output of format FMT; `lanes` of a block of 32 elements are 32 / V neighbours and all of them call
-template <typename T, int V, int FMT>
-DEV void put(const dist_rms_args& p, const float y[V], float inv, long row, long c, int Kp) {
-    if constexpr (FMT == DIST_RMS_SAME) {
-        if (c < p.C) mx::store_v<V>(static_cast<T*>(p.y) + row * p.ldy + c, y);
-    } else if constexpr (FMT == DIST_RMS_E4M3) {
+// eight neighbouring values of a row from column c on -> the output of format FMT; the four lanes of a block of 32 are neighbours and all of them call
+template <typename T, bool AL, int FMT>
+DEV void put(const dist_rms_args& p, const float y[8], float inv, long row, long c, int Kp) {
+    const long left = p.C - c;
+    if constexpr (FMT == DIST_RMS_SAME) mx::store8<AL>(static_cast<T*>(p.y) + row * p.ldy + c, left, y);
+    else if constexpr (FMT == DIST_RMS_E4M3) {
+        int lo = 0, hi = 0;
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * inv, y[1] * inv, lo, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * inv, y[3] * inv, lo, true);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4] * inv, y[5] * inv, hi, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6] * inv, y[7] * inv, hi, true);
         unsigned char* q = static_cast<unsigned char*>(p.y) + row * p.ldy + c;
-        if constexpr (V == 8) {
-            if (c < p.C) {
-                int lo = 0, hi = 0;
-                lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * inv, y[1] * inv, lo, false);
-                lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * inv, y[3] * inv, lo, true);
-                hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4] * inv, y[5] * inv, hi, false);
-                hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6] * inv, y[7] * inv, hi, true);
-                *reinterpret_cast<int2*>(q) = make_int2(lo, hi);
+        if constexpr (AL) {
+            const mx::i32x2_t w = {lo, hi};
+            if (left > 0) __builtin_nontemporal_store(w, reinterpret_cast<mx::i32x2_t*>(q));
+        } else {
+            const unsigned long w = (unsigned)lo | (unsigned long)(unsigned)hi << 32;
+            if (left >= 8) __builtin_memcpy(q, &w, 8);
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < left) q[e] = (unsigned char)(w >> (8 * e));
             }
-        } else if (c < p.C) *q = (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(y[0] * inv, 0.f, 0, false) & 0xff);
+        }
     } else {
         unsigned a = 0;
 #pragma unroll
-        for (int e = 0; e < V; ++e) a = max(a, mx::abs_bits(y[e]));
-#pragma unroll
-        for (int o = 1; o < 32 / V; o *= 2) a = max(a, (unsigned)__shfl_xor((int)a, o, 64));
+        for (int e = 0; e < 8; ++e) a = max(a, mx::abs_bits(y[e]));
+        a = max(a, (unsigned)__shfl_xor((int)a, 1, 64));
+        a = max(a, (unsigned)__shfl_xor((int)a, 2, 64));
         const int byte = mx::scale_byte(a);
-        unsigned char* q = static_cast<unsigned char*>(p.y) + row * (Kp / 2) + c / 2;
-        if constexpr (V == 8) {
-            if (c < Kp) *reinterpret_cast<unsigned*>(q) = mx::pack8(y, byte);
-        } else {
-            const float other = __shfl_xor(y[0], 1, 64);
-            if (c < Kp && (c & 1) == 0)
-                *q = byte == 255 ? 0 : (unsigned char)(__builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], other, mx::scale_value(byte), 0) & 0xff);
-        }
+        if (c < Kp) *reinterpret_cast<unsigned*>(static_cast<unsigned char*>(p.y) + row * (Kp / 2) + c / 2) = mx::pack8(y, byte);
         if (c % 32 == 0 && c < (long)(Kp + 255) / 256 * 256) static_cast<unsigned char*>(p.scale)[mx::scale_at(row, p.rows, (int)(c / 32))] = (unsigned char)(c < Kp ? byte : 0);
     }
 }
 
-// LPR lanes own a row and hold IT groups of V elements each (V = 8: aligned rows of whole groups; V = 1: any width and alignment)
-template <typename T, int V, int LPR, int IT, int FMT>
+// LPR lanes own a row and hold IT groups of eight elements each
+template <typename T, bool AL, int LPR, int IT, int FMT>
 __global__ __launch_bounds__(NT) void rms_fwd_kernel(const dist_rms_args p) {
     __shared__ float red[4];
     const int lr = threadIdx.x % LPR;
@@ -81,50 +81,44 @@ __global__ __launch_bounds__(NT) void rms_fwd_kernel(const dist_rms_args p) {
     const int C = p.C, Kp = (C + 31) / 32 * 32;
     const T* X = static_cast<const T*>(p.x) + row * p.ldx;
     const T* R = p.res ? static_cast<const T*>(p.res) + row * p.ldres : nullptr;
-    float x[IT][V];
+    float x[IT][8];
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
-        const int c = (lr + it * LPR) * V;
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[it][e] = 0.f;
-        if (c < C) mx::load_v<V>(X + c, x[it]);
+        const int c = (lr + it * LPR) * 8;
+        mx::load8<AL>(X + c, C - c, x[it]);
     }
     if (R) {
 #pragma unroll
         for (int it = 0; it < IT; ++it) {
-            const int c = (lr + it * LPR) * V;
-            if (c < C) {
-                float r[V];
-                mx::load_v<V>(R + c, r);
+            const int c = (lr + it * LPR) * 8;
+            float r[8];
+            mx::load8<AL>(R + c, C - c, r);
 #pragma unroll
-                for (int e = 0; e < V; ++e) x[it][e] += r[e];
-            }
+            for (int e = 0; e < 8; ++e) x[it][e] += r[e];
         }
     }
     float s = 0.f;
 #pragma unroll
     for (int it = 0; it < IT; ++it)
 #pragma unroll
-        for (int e = 0; e < V; ++e) s += x[it][e] * x[it][e];
+        for (int e = 0; e < 8; ++e) s += x[it][e] * x[it][e];
     const float rstd = 1.f / sqrtf(row_sum<LPR>(s, red) / (float)C + p.eps);
     if (p.rstd && lr == 0) p.rstd[row] = rstd;
     if (p.h) {
         T* H = static_cast<T*>(p.h) + row * p.ldh;
 #pragma unroll
         for (int it = 0; it < IT; ++it) {
-            const int c = (lr + it * LPR) * V;
-            if (c < C) mx::store_v<V>(H + c, x[it]);
+            const int c = (lr + it * LPR) * 8;
+            mx::store8<AL>(H + c, C - c, x[it]);
         }
     }
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
-        const int c = (lr + it * LPR) * V;
-        if (c < C) {
-            float w[V];
-            mx::load_v<V>(p.w + c, w);
+        const int c = (lr + it * LPR) * 8;
+        float w[8];
+        mx::load8<AL>(p.w + c, C - c, w);
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[it][e] = x[it][e] * rstd * w[e];
-        }
+        for (int e = 0; e < 8; ++e) x[it][e] = AL || c + e < C ? x[it][e] * rstd * w[e] : 0.f;
     }
     float inv = 1.f;
     if constexpr (FMT == DIST_RMS_E4M3) {
@@ -132,12 +126,12 @@ __global__ __launch_bounds__(NT) void rms_fwd_kernel(const dist_rms_args p) {
 #pragma unroll
         for (int it = 0; it < IT; ++it)
 #pragma unroll
-            for (int e = 0; e < V; ++e) a = fmaxf(a, fabsf(x[it][e]));
+            for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(x[it][e]));
         inv = e4m3_factor(row_max<LPR>(a, red), scale);
         if (lr == 0) static_cast<float*>(p.scale)[row] = scale;
     }
 #pragma unroll
-    for (int it = 0; it < IT; ++it) put<T, V, FMT>(p, x[it], inv, row, (long)(lr + it * LPR) * V, Kp);
+    for (int it = 0; it < IT; ++it) put<T, AL, FMT>(p, x[it], inv, row, (long)(lr + it * LPR) * 8, Kp);
 }
 
 // rows too long for the registers: the block walks its row again for every step (the second and third walk find it in the L2).  h is stored last, so it may be x or res.
@@ -145,66 +139,104 @@ template <typename T, int FMT>
 __global__ __launch_bounds__(NT) void rms_fwd_long_kernel(const dist_rms_args p) {
     __shared__ float red[4];
     const long row = blockIdx.x;
-    const int C = p.C, Kp = (C + 31) / 32 * 32, tid = threadIdx.x;
+    const int C = p.C, Kp = (C + 31) / 32 * 32;
     const T* X = static_cast<const T*>(p.x) + row * p.ldx;
     const T* R = p.res ? static_cast<const T*>(p.res) + row * p.ldres : nullptr;
     T* H = p.h ? static_cast<T*>(p.h) + row * p.ldh : nullptr;
-    float s = 0.f;
-    for (long c = tid; c < C; c += NT) { const float h = to_f(X[c]) + (R ? to_f(R[c]) : 0.f); s += h * h; }
+    auto group = [&](long c, float h[8]) __attribute__((always_inline)) {
+        float r[8];
+        mx::load8<false>(X + c, C - c, h);
+        if (!R) return;
+        mx::load8<false>(R + c, C - c, r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] += r[e];
+    };
+    auto norm = [&](long c, float h[8], float rstd) __attribute__((always_inline)) {
+        float w[8];
+        mx::load8<false>(p.w + c, C - c, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = c + e < C ? h[e] * rstd * w[e] : 0.f;
+    };
+    float s = 0.f, h[8];
+    for (long c = threadIdx.x * 8; c < C; c += NT * 8) {
+        group(c, h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += h[e] * h[e];
+    }
     const float rstd = 1.f / sqrtf(row_sum<NT>(s, red) / (float)C + p.eps);
-    if (p.rstd && tid == 0) p.rstd[row] = rstd;
+    if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
     float inv = 1.f;
     if constexpr (FMT == DIST_RMS_E4M3) {
         float a = 0.f, scale;
-        for (long c = tid; c < C; c += NT) a = fmaxf(a, fabsf((to_f(X[c]) + (R ? to_f(R[c]) : 0.f)) * rstd * p.w[c]));
-        inv = e4m3_factor(row_max<NT>(a, red), scale);
-        if (tid == 0) static_cast<float*>(p.scale)[row] = scale;
-    }
-    for (long c = tid; c < ((long)C + NT - 1) / NT * NT; c += NT) {          // (whole chunks: every lane of a block of 32 takes part)
-        float y = 0.f;
-        if (c < C) {
-            const float h = to_f(X[c]) + (R ? to_f(R[c]) : 0.f);
-            y = h * rstd * p.w[c];
-            if (H) H[c] = from_f<T>(h);
+        for (long c = threadIdx.x * 8; c < C; c += NT * 8) {
+            group(c, h);
+            norm(c, h, rstd);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(h[e]));
         }
-        put<T, 1, FMT>(p, &y, inv, row, c, Kp);
+        inv = e4m3_factor(row_max<NT>(a, red), scale);
+        if (threadIdx.x == 0) static_cast<float*>(p.scale)[row] = scale;
+    }
+    for (long c = threadIdx.x * 8; c < ((long)C + NT * 8 - 1) / (NT * 8) * (NT * 8); c += NT * 8) {          // (every lane of a block of 32 takes part)
+        group(c, h);
+        if (H) mx::store8<false>(H + c, C - c, h);
+        norm(c, h, rstd);
+        put<T, false, FMT>(p, h, inv, row, c, Kp);
     }
 }
 
 // Backward.  A block keeps the sums of dw over its rows in registers and leaves one partial row; rms_dw_kernel adds the partial rows in a fixed order (no atomics:
 // the same bits every time).
-template <typename T, typename TD, int V, int LPR, int IT>
+template <typename T, typename TD, bool AL, int LPR, int IT>
 __global__ __launch_bounds__(NT) void rms_bwd_kernel(const dist_rms_bwd_args p) {
     __shared__ float red[4];
-    __shared__ float cols[LPR < NT ? LPR * IT * V : 1];
+    __shared__ float cols[LPR < NT ? LPR * IT * 8 : 1];
     const int lr = threadIdx.x % LPR, slot = threadIdx.x / LPR, C = p.C;
     constexpr int RPB = NT / LPR;
-    float w[IT][V], aw[IT][V];
+    float w[IT][8], aw[IT][8];
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
-        const int c = (lr + it * LPR) * V;
+        const int c = (lr + it * LPR) * 8;
+        mx::load8<AL>(p.w + c, C - c, w[it]);
 #pragma unroll
-        for (int e = 0; e < V; ++e) w[it][e] = aw[it][e] = 0.f;
-        if (c < C) mx::load_v<V>(p.w + c, w[it]);
+        for (int e = 0; e < 8; ++e) aw[it][e] = 0.f;
     }
-    for (long row = (long)blockIdx.x * RPB + slot; row < p.rows; row += (long)gridDim.x * RPB) {
-        const T* H = static_cast<const T*>(p.h) + row * p.ldh;
-        const TD* D = static_cast<const TD*>(p.dy) + row * p.lddy;
-        const float rstd = p.rstd[row];
-        float n[IT][V], g[IT][V];
+    // the next row is read while this one is worked on (50432 x 768 bf16 with dres: 77 us without, 62 with)
+    const T* const A = static_cast<const T*>(p.dres);
+    mx::Raw8<AL, T> hn[IT], rn[IT];
+    mx::Raw8<AL, TD> dn[IT];
+    float sn = 0.f;
+    auto fetch = [&](long row) __attribute__((always_inline)) {
+        row = min(row, p.rows - 1);
 #pragma unroll
         for (int it = 0; it < IT; ++it) {
-            const int c = (lr + it * LPR) * V;
-#pragma unroll
-            for (int e = 0; e < V; ++e) n[it][e] = g[it][e] = 0.f;
-            if (c < C) { mx::load_v<V>(H + c, n[it]); mx::load_v<V>(D + c, g[it]); }
+            const int c = (lr + it * LPR) * 8;
+            hn[it].load(static_cast<const T*>(p.h) + row * p.ldh + c, C - c);
+            dn[it].load(static_cast<const TD*>(p.dy) + row * p.lddy + c, C - c);
+            if (A) rn[it].load(A + row * p.lddres + c, C - c);
         }
+        sn = p.rstd[row];
+    };
+    const long stride = (long)gridDim.x * RPB;
+    long row = (long)blockIdx.x * RPB + slot;
+    if (row < p.rows) fetch(row);
+    for (; row < p.rows; row += stride) {
+        const float rstd = sn;
+        float n[IT][8], g[IT][8], o[IT][8];
+#pragma unroll
+        for (int it = 0; it < IT; ++it)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                n[it][e] = hn[it].get(e) * rstd;
+                g[it][e] = dn[it].get(e);
+                o[it][e] = A ? rn[it].get(e) : 0.f;
+            }
+        if (row + stride < p.rows) fetch(row + stride);
         float s = 0.f;
 #pragma unroll
         for (int it = 0; it < IT; ++it)
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                n[it][e] *= rstd;
+            for (int e = 0; e < 8; ++e) {
                 aw[it][e] += g[it][e] * n[it][e];
                 g[it][e] *= w[it][e];
                 s += g[it][e] * n[it][e];
@@ -212,19 +244,12 @@ __global__ __launch_bounds__(NT) void rms_bwd_kernel(const dist_rms_bwd_args p) 
         const float m = row_sum<LPR>(s, red) / (float)C;
         if (p.dh) {
             T* O = static_cast<T*>(p.dh) + row * p.lddh;
-            const T* A = p.dres ? static_cast<const T*>(p.dres) + row * p.lddres : nullptr;
 #pragma unroll
             for (int it = 0; it < IT; ++it) {
-                const int c = (lr + it * LPR) * V;
-                if (c < C) {
-                    float o[V], a[V];
+                const int c = (lr + it * LPR) * 8;
 #pragma unroll
-                    for (int e = 0; e < V; ++e) a[e] = 0.f;
-                    if (A) mx::load_v<V>(A + c, a);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) o[e] = rstd * (g[it][e] - n[it][e] * m) + a[e];
-                    mx::store_v<V>(O + c, o);
-                }
+                for (int e = 0; e < 8; ++e) o[it][e] = rstd * (g[it][e] - n[it][e] * m) + o[it][e];
+                mx::store8<AL>(O + c, C - c, o[it]);
             }
         }
     }
@@ -232,10 +257,10 @@ __global__ __launch_bounds__(NT) void rms_bwd_kernel(const dist_rms_bwd_args p) 
     if constexpr (LPR == NT) {
 #pragma unroll
         for (int it = 0; it < IT; ++it) {
-            const int c = (lr + it * LPR) * V;
-            if (c < C)
+            const int c = (lr + it * LPR) * 8;
 #pragma unroll
-                for (int e = 0; e < V; ++e) part[c + e] = aw[it][e];
+            for (int e = 0; e < 8; ++e)
+                if (c + e < C) part[c + e] = aw[it][e];
         }
     } else {
         for (int k = 0; k < RPB; ++k) {                                       // the block's row slots, one after the other
@@ -243,9 +268,9 @@ __global__ __launch_bounds__(NT) void rms_bwd_kernel(const dist_rms_bwd_args p) 
 #pragma unroll
                 for (int it = 0; it < IT; ++it)
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        float& o = cols[(lr + it * LPR) * V + e];
-                        o = k == 0 ? aw[it][e] : o + aw[it][e];
+                    for (int e = 0; e < 8; ++e) {
+                        float& q = cols[(lr + it * LPR) * 8 + e];
+                        q = k == 0 ? aw[it][e] : q + aw[it][e];
                     }
             }
             __syncthreads();
@@ -281,61 +306,49 @@ __global__ __launch_bounds__(NT) void rms_dw_cols_kernel(const dist_rms_bwd_args
     p.scratch[(long)slice * p.C + c] = s;
 }
 
-// dw[c] (+)= sum of the partial rows: 16 groups of 64 threads take every 16th row each, then the groups in order
+// dw[c] (+)= sum of the partial rows: 64 groups of 16 threads take every 64th row each, then the groups in order
 __global__ __launch_bounds__(1024) void rms_dw_kernel(const float* __restrict__ part, const int G, const int C, float* __restrict__ dw, const int accumulate) {
-    __shared__ float red[16][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6;
+    __shared__ float red[64][16];
+    const int l = threadIdx.x & 15, c = blockIdx.x * 16 + l, g = threadIdx.x >> 4;
     float s = 0.f;
     if (c < C) {
 #pragma unroll 8
-        for (int k = g; k < G; k += 16) s += part[(long)k * C + c];
+        for (int k = g; k < G; k += 64) s += part[(long)k * C + c];
     }
-    red[g][threadIdx.x & 63] = s;
+    red[g][l] = s;
     __syncthreads();
     if (g == 0 && c < C) {
-#pragma unroll
-        for (int k = 1; k < 16; ++k) s += red[k][threadIdx.x];
+#pragma unroll 8
+        for (int k = 1; k < 64; ++k) s += red[k][l];
         dw[c] = accumulate ? dw[c] + s : s;
     }
 }
 
-constexpr int VEC_MAX = 16384, ONE_MAX = 4096;                 // widths the register-resident kernels take
-constexpr int BWD_VEC_MAX = 8192, BWD_ONE_MAX = 4096;
+constexpr int FWD_MAX = 16384, BWD_MAX = 8192;                // widths whose rows stay in registers
+constexpr int PARTIALS = 512;                                  // workgroups of the backward kernel, two a CU (50432 x 768: 384 67 us, 512 62, 640 77, 1024 66)
 
-// lanes per row of the backward kernel for this width and vector length (0: a long row)
-inline int bwd_lanes(int C, bool vec) {
-    if (vec) return C <= 384 ? 16 : C <= 768 ? 32 : C <= 2048 ? 64 : C <= BWD_VEC_MAX ? 256 : 0;
-    return C <= 1024 ? 64 : C <= BWD_ONE_MAX ? 256 : 0;
-}
-inline int64_t bwd_partials(int64_t rows, int C, bool vec) {
-    const int lanes = bwd_lanes(C, vec);
-    if (!lanes) return rows < 64 ? (rows < 1 ? 1 : rows) : 64;
-    const int64_t need = (rows + NT / lanes - 1) / (NT / lanes);
-    return need < 1 ? 1 : need > 1024 ? 1024 : need;
+// lanes per row of the backward kernel (0: a long row)
+inline int bwd_lanes(int C) { return C <= 384 ? 16 : C <= 768 ? 32 : C <= 2048 ? 64 : C <= BWD_MAX ? 256 : 0; }
+inline int64_t bwd_partials(int64_t rows, int C) {
+    const int lanes = bwd_lanes(C);
+    const int64_t need = lanes ? (rows + NT / lanes - 1) / (NT / lanes) : rows, most = lanes ? PARTIALS : 64;
+    return need < 1 ? 1 : need > most ? most : need;
 }
 inline bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
-template <typename T, int FMT> int fwd(const dist_rms_args& p, hipStream_t s) {
-    bool vec = p.C % 8 == 0 && p.ldx % 8 == 0 && aligned16(p.x) && aligned16(p.w) && (!p.res || (p.ldres % 8 == 0 && aligned16(p.res))) &&
-               (!p.h || (p.ldh % 8 == 0 && aligned16(p.h))) && aligned16(p.y);
-    if (FMT != DIST_RMS_MXFP4) vec = vec && p.ldy % 8 == 0;
+template <typename T, bool AL, int FMT> int fwd(const dist_rms_args& p, hipStream_t s) {
     const int64_t Cr = FMT == DIST_RMS_MXFP4 ? ((int64_t)p.C + 255) / 256 * 256 : p.C;       // (the scale bytes of a whole chunk are written)
     const int64_t rows = p.rows;
-#define DIST_RMS(V, LPR, IT) do { const int64_t b = (rows + NT / LPR - 1) / (NT / LPR); if (b > 0x7fffffff) return DIST_ERR_ARG; \
-        hipLaunchKernelGGL((rms_fwd_kernel<T, V, LPR, IT, FMT>), dim3((unsigned)b), dim3(NT), 0, s, p); } while (0)
-    if (vec && Cr <= VEC_MAX) {
-        if (Cr <= 384) DIST_RMS(8, 16, 3);
-        else if (Cr <= 768) DIST_RMS(8, 32, 3);
-        else if (Cr <= 1024) DIST_RMS(8, 64, 2);
-        else if (Cr <= 2048) DIST_RMS(8, 64, 4);
-        else if (Cr <= 4096) DIST_RMS(8, 256, 2);
-        else if (Cr <= 8192) DIST_RMS(8, 256, 4);
-        else DIST_RMS(8, 256, 8);
-    } else if (Cr <= ONE_MAX) {
-        if (Cr <= 1024) DIST_RMS(1, 64, 16);
-        else if (Cr <= 2048) DIST_RMS(1, 256, 8);
-        else DIST_RMS(1, 256, 16);
-    } else {
+#define DIST_RMS(LPR, IT) do { const int64_t b = (rows + NT / LPR - 1) / (NT / LPR); if (b > 0x7fffffff) return DIST_ERR_ARG; \
+        hipLaunchKernelGGL((rms_fwd_kernel<T, AL, LPR, IT, FMT>), dim3((unsigned)b), dim3(NT), 0, s, p); } while (0)
+    if (Cr <= 384) DIST_RMS(16, 3);
+    else if (Cr <= 768) DIST_RMS(32, 3);
+    else if (Cr <= 1024) DIST_RMS(64, 2);
+    else if (Cr <= 2048) DIST_RMS(64, 4);
+    else if (Cr <= 4096) DIST_RMS(256, 2);
+    else if (Cr <= 8192) DIST_RMS(256, 4);
+    else if (Cr <= FWD_MAX) DIST_RMS(256, 8);
+    else {
         if (rows > 0x7fffffff) return DIST_ERR_ARG;
         hipLaunchKernelGGL((rms_fwd_long_kernel<T, FMT>), dim3((unsigned)rows), dim3(NT), 0, s, p);
     }
@@ -343,30 +356,35 @@ template <typename T, int FMT> int fwd(const dist_rms_args& p, hipStream_t s) {
     HIP_CHECK_RET(hipGetLastError());
     return DIST_OK;
 }
+template <typename T, int FMT> int fwd(const dist_rms_args& p, hipStream_t s) {
+    const bool al = p.C % 8 == 0 && p.ldx % 8 == 0 && aligned16(p.x) && aligned16(p.w) && (!p.res || (p.ldres % 8 == 0 && aligned16(p.res))) &&
+                    (!p.h || (p.ldh % 8 == 0 && aligned16(p.h))) && aligned16(p.y) && (FMT == DIST_RMS_MXFP4 || p.ldy % 8 == 0);
+    return al ? fwd<T, true, FMT>(p, s) : fwd<T, false, FMT>(p, s);
+}
 
-template <typename T, typename TD> int bwd(const dist_rms_bwd_args& p, bool vec, hipStream_t s) {
-    const int G = (int)bwd_partials(p.rows, p.C, vec);
-    const int lanes = bwd_lanes(p.C, vec);
-#define DIST_RMS(V, LPR, IT) hipLaunchKernelGGL((rms_bwd_kernel<T, TD, V, LPR, IT>), dim3((unsigned)G), dim3(NT), 0, s, p)
+template <typename T, typename TD, bool AL> int bwd(const dist_rms_bwd_args& p, hipStream_t s) {
+    const int G = (int)bwd_partials(p.rows, p.C);
+    const int lanes = bwd_lanes(p.C);
+#define DIST_RMS(LPR, IT) hipLaunchKernelGGL((rms_bwd_kernel<T, TD, AL, LPR, IT>), dim3((unsigned)G), dim3(NT), 0, s, p)
     if (!lanes) {
         if (p.rows > 0x7fffffff) return DIST_ERR_ARG;
         const int ctiles = (p.C + NT - 1) / NT;
         if (p.dh && p.rows) hipLaunchKernelGGL((rms_bwd_long_kernel<T, TD>), dim3((unsigned)p.rows), dim3(NT), 0, s, p);
         hipLaunchKernelGGL((rms_dw_cols_kernel<T, TD>), dim3((unsigned)(G * ctiles)), dim3(NT), 0, s, p, G, ctiles);
-    } else if (vec) {
-        if (lanes == 16) DIST_RMS(8, 16, 3);
-        else if (lanes == 32) DIST_RMS(8, 32, 3);
-        else if (lanes == 64) { if (p.C <= 1024) DIST_RMS(8, 64, 2); else DIST_RMS(8, 64, 4); }
-        else { if (p.C <= 4096) DIST_RMS(8, 256, 2); else DIST_RMS(8, 256, 4); }
-    } else {
-        if (lanes == 64) DIST_RMS(1, 64, 16);
-        else DIST_RMS(1, 256, 16);
-    }
+    } else if (lanes == 16) DIST_RMS(16, 3);
+    else if (lanes == 32) DIST_RMS(32, 3);
+    else if (lanes == 64) { if (p.C <= 1024) DIST_RMS(64, 2); else DIST_RMS(64, 4); }
+    else { if (p.C <= 4096) DIST_RMS(256, 2); else DIST_RMS(256, 4); }
 #undef DIST_RMS
     HIP_CHECK_RET(hipGetLastError());
-    hipLaunchKernelGGL(rms_dw_kernel, dim3((unsigned)((p.C + 63) / 64)), dim3(1024), 0, s, p.scratch, G, p.C, p.dw, p.accumulate);
+    hipLaunchKernelGGL(rms_dw_kernel, dim3((unsigned)((p.C + 15) / 16)), dim3(1024), 0, s, p.scratch, G, p.C, p.dw, p.accumulate);
     HIP_CHECK_RET(hipGetLastError());
     return DIST_OK;
+}
+template <typename T, typename TD> int bwd(const dist_rms_bwd_args& p, hipStream_t s) {
+    const bool al = p.C % 8 == 0 && p.ldh % 8 == 0 && p.lddy % 8 == 0 && aligned16(p.h) && aligned16(p.dy) && aligned16(p.w) &&
+                    (!p.dres || (p.lddres % 8 == 0 && aligned16(p.dres))) && (!p.dh || (p.lddh % 8 == 0 && aligned16(p.dh)));
+    return al ? bwd<T, TD, true>(p, s) : bwd<T, TD, false>(p, s);
 }
 
 }  // namespace
@@ -390,8 +408,7 @@ extern "C" int dist_op_rmsnorm(const dist_rms_args* a, void* stream) {
 
 extern "C" int64_t dist_op_rmsnorm_bwd_scratch(int64_t rows, int C) {
     if (rows < 0 || C <= 0) return -1;
-    const int64_t a = bwd_partials(rows, C, true), b = bwd_partials(rows, C, false);
-    return (a > b ? a : b) * C;
+    return bwd_partials(rows, C) * C;
 }
 
 extern "C" int dist_op_rmsnorm_bwd(const dist_rms_bwd_args* a, void* stream) {
@@ -403,9 +420,7 @@ extern "C" int dist_op_rmsnorm_bwd(const dist_rms_bwd_args* a, void* stream) {
     if (p.rows > 0 && (!p.h || !p.rstd || !p.dy || p.ldh < p.C || p.lddy < p.C || (p.dres && p.lddres < p.C) || (p.dh && p.lddh < p.C))) return DIST_ERR_ARG;
     const uintptr_t es = p.dtype == DIST_BF16 ? 2 : 4, ed = p.dy_dtype == DIST_BF16 ? 2 : 4;
     if ((uintptr_t)p.h % es || (uintptr_t)p.dres % es || (uintptr_t)p.dh % es || (uintptr_t)p.dy % ed) return DIST_ERR_ARG;
-    const bool vec = p.C % 8 == 0 && p.ldh % 8 == 0 && p.lddy % 8 == 0 && aligned16(p.h) && aligned16(p.dy) && aligned16(p.w) &&
-                     (!p.dres || (p.lddres % 8 == 0 && aligned16(p.dres))) && (!p.dh || (p.lddh % 8 == 0 && aligned16(p.dh)));
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (p.dtype == DIST_BF16) return p.dy_dtype == DIST_BF16 ? bwd<bf16_t, bf16_t>(p, vec, s) : bwd<bf16_t, float>(p, vec, s);
-    return p.dy_dtype == DIST_BF16 ? bwd<float, bf16_t>(p, vec, s) : bwd<float, float>(p, vec, s);
+    if (p.dtype == DIST_BF16) return p.dy_dtype == DIST_BF16 ? bwd<bf16_t, bf16_t>(p, s) : bwd<bf16_t, float>(p, s);
+    return p.dy_dtype == DIST_BF16 ? bwd<float, bf16_t>(p, s) : bwd<float, float>(p, s);
 }
