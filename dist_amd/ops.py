@@ -552,6 +552,7 @@ def attention_fp8(qkv8, in_scale, frames, Ltok, heads, out8_scale=None, amax=Non
 # ---- a 4-bit frozen linear layer: norm, microscaled 4-bit quantisation, product ---------------------------------------------------------------------------------
 # (One token's call is bound by this host code: checks are plain comparisons, messages are made only when one fails, and the launch takes the raw stream of the
 # operands' GPU - 0.1 us against 2.8 us for torch.cuda.current_stream().)
+_LONGEST = 1 << 30                # what the library takes as a width (a C int)
 RMS_FMTS = {"same": L.RMS_SAME, "e4m3": L.RMS_E4M3, "mxfp4": L.RMS_MXFP4}
 
 
@@ -616,6 +617,11 @@ def _apart(out, what, *inputs, may_be=True):
             _refuse(f"{what} overlaps an input without being it")
 
 
+def _new(like, dense, dtype):
+    """a contiguous tensor of the same shape (empty_like is the faster call, and contiguous where its model is)"""
+    return torch.empty_like(like, dtype=dtype) if dense else torch.empty(like.shape, dtype=dtype, device=like.device)
+
+
 def _mx_empty(rows, K, device):
     """buffers of an MXFP4 operand of `rows` rows of K elements: (codes [rows, Kp / 2], scales [chunks, rows, 8]), uint8"""
     return torch.empty(rows, (K + 31) // 32 * 16, dtype=torch.uint8, device=device), torch.empty((K + 255) // 256, rows, 8, dtype=torch.uint8, device=device)
@@ -645,8 +651,8 @@ def rmsnorm(x, w, *, res=None, fmt="same", h=None, rstd=None, eps=1e-6):
         _refuse(f"fmt {fmt!r}: one of {sorted(RMS_FMTS)}")
     dtype, shape = x.dtype, x.shape
     dt = _dt(x)
-    if len(shape) != 2 or shape[1] == 0:
-        _refuse(f"x: expected [rows, C] with C > 0, got {tuple(shape)}")
+    if len(shape) != 2 or not 0 < shape[1] <= _LONGEST:
+        _refuse(f"x: expected [rows, C] with 0 < C <= {_LONGEST}, got {tuple(shape)}")
     rows, Cc = shape
     ldx = _matrix(x, shape, "x", dtype)
     _vector(w, Cc, "w")
@@ -654,19 +660,19 @@ def rmsnorm(x, w, *, res=None, fmt="same", h=None, rstd=None, eps=1e-6):
         _vector(rstd, rows, "rstd")
     ldres = _matrix(res, shape, "res", dtype) if res is not None else 0
     dev = _device(x, w, res, h, rstd)
-    out = {}
+    out, dense = {}, x.is_contiguous()
     if h is not None:
         ldh = _matrix(h, shape, "h", dtype)
         _apart(h, "h", x, res)
     elif res is not None:
-        h, ldh = torch.empty(shape, dtype=dtype, device=x.device), Cc
+        h, ldh = _new(x, dense, dtype), Cc
     if h is not None:
         out["h"] = h
     if code == L.RMS_SAME:
-        y, sc = torch.empty(shape, dtype=dtype, device=x.device), None
+        y, sc = _new(x, dense, dtype), None
         out["y"] = y
     elif code == L.RMS_E4M3:
-        y, sc = torch.empty(shape, dtype=torch.uint8, device=x.device), torch.empty(rows, dtype=torch.float32, device=x.device)
+        y, sc = _new(x, dense, torch.uint8), torch.empty(rows, dtype=torch.float32, device=x.device)
         out["q"], out["scale"] = y, sc
     else:
         y, sc = _mx_empty(rows, Cc, x.device)
@@ -682,8 +688,8 @@ def rmsnorm_bwd(h, rstd, dy, w, *, dres=None, dh=None, dw=None):
     dh: a buffer for the result (it may be dres, h or dy itself); dw (fp32 [C]) is ACCUMULATED into when given.  Returns (dh, dw).  The same bits every time."""
     dt, dyt = _dt(h), _dt(dy)
     dtype, shape = h.dtype, h.shape
-    if len(shape) != 2 or shape[1] == 0:
-        _refuse(f"h: expected [rows, C] with C > 0, got {tuple(shape)}")
+    if len(shape) != 2 or not 0 < shape[1] <= _LONGEST:
+        _refuse(f"h: expected [rows, C] with 0 < C <= {_LONGEST}, got {tuple(shape)}")
     rows, Cc = shape
     ldh, lddy = _matrix(h, shape, "h", dtype), _matrix(dy, shape, "dy", dy.dtype)
     _vector(w, Cc, "w")
@@ -691,7 +697,7 @@ def rmsnorm_bwd(h, rstd, dy, w, *, dres=None, dh=None, dw=None):
     lddres = _matrix(dres, shape, "dres", dtype) if dres is not None else 0
     dev = _device(h, rstd, dy, w, dres, dh, dw)
     if dh is None:
-        dh, lddh = torch.empty(shape, dtype=dtype, device=h.device), Cc
+        dh, lddh = _new(h, h.is_contiguous(), dtype), Cc
     else:
         lddh = _matrix(dh, shape, "dh", dtype)
         _apart(dh, "dh", h, dy, dres)
@@ -741,8 +747,8 @@ def gemm_mxfp4(A, B, *, bias=None, res=None, out=None, out_dtype=torch.bfloat16)
     C is bf16, or fp32 with an MXFP4 A.  The gradients are the same call: dA = gemm_mxfp4(quant_mxfp4(dC), quant_mxfp4(W, transpose=True)),
     dW = gemm_mxfp4(quant_mxfp4(dC, transpose=True), quant_mxfp4(X, transpose=True))."""
     N, K = _mx_operand(B, "B")
-    if N == 0:
-        _refuse("B has no rows")
+    if not 0 < N <= _LONGEST or K > _LONGEST:
+        _refuse(f"B: expected 1 to {_LONGEST} rows of at most as many elements, got {N} x {K}")
     if not isinstance(A, (tuple, list)) or len(A) != 2:
         _refuse("A: expected a pair (codes, scales) or (q, scale)")
     q, sc = A

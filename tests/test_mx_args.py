@@ -59,7 +59,8 @@ def test_rmsnorm_bwd_scratch_is_checked():
 
 
 @pytest.mark.parametrize("args", [(None, 1, 4, 64, 64, 0, P, P), (P, 1, 4, 64, 64, 0, None, P), (P, 1, 4, 64, 64, 0, P, None), (P, 5, 4, 64, 64, 0, P, P), (P, 1, 4, 64, 63, 0, P, P),
-                                  (P, 1, -1, 64, 64, 0, P, P), (P, 1, 4, 0, 0, 0, P, P), (P, 1, 0, 64, 64, 1, P, P), (P, 1, 4, 64, 64, 0, P + 8, P), (P + 1, 1, 4, 64, 64, 0, P, P)])
+                                  (P, 1, -1, 64, 64, 0, P, P), (P, 1, 4, 0, 0, 0, P, P), (P, 1, 0, 64, 64, 1, P, P), (P, 1, 4, 64, 64, 0, P + 8, P), (P + 1, 1, 4, 64, 64, 0, P, P),
+                                  (P, 1, 4, 64, 64, 0, P, P + 4)])
 def test_quant_refuses(args):
     assert L.load().dist_op_quant_mxfp4(*args, None) == -1
 
@@ -78,10 +79,19 @@ def _gemm(**kw):
 
 
 @pytest.mark.parametrize("kw", [dict(A=None), dict(a_scale=None), dict(B=None), dict(b_scale=None), dict(C=None), dict(M=-1), dict(N=0), dict(K=0), dict(K=48), dict(ldc=7),
-                                dict(res=P, ldres=7), dict(a_fmt=2), dict(dtype=2), dict(a_fmt=L.MX_A_E4M3, dtype=L.F32), dict(a_fmt=L.MX_A_E4M3, lda=63), dict(a_fmt=L.MX_A_E4M3, lda=72),
+                                dict(res=P, ldres=7), dict(a_fmt=2), dict(dtype=2), dict(a_fmt=L.MX_A_E4M3, dtype=L.F32), dict(a_fmt=L.MX_A_E4M3, lda=63), dict(a_fmt=L.MX_A_E4M3, lda=72), dict(K=(1 << 22) + 32), dict(a_fmt=L.MX_A_E4M3, lda=(1 << 22) + 16),
                                 dict(A=P + 8), dict(B=P + 8), dict(b_scale=P + 4), dict(a_scale=P + 4), dict(C=P + 1), dict(bias=P + 2)])
 def test_gemm_refuses(kw):
     assert _gemm(**kw) == -1
+
+
+def test_gemm_scratch_is_checked():
+    """a long axis over few tiles is cut into slices, whose partial results need a place"""
+    l = L.load()
+    n = l.dist_op_gemm_mxfp4_scratch(128, 128, 16384, L.MX_A_MXFP4)
+    assert n > 0 and n % (128 * 128) == 0 and l.dist_op_gemm_mxfp4_scratch(64, 128, 16384, L.MX_A_MXFP4) == 0 and l.dist_op_gemm_mxfp4_scratch(50432, 2304, 768, L.MX_A_E4M3) == 0
+    big = dict(M=128, N=128, K=16384, ldc=128)
+    assert _gemm(**big) == -3 and _gemm(**big, scratch=P, scratch_elems=n - 1) == -3 and _gemm(**big, scratch=P + 4, scratch_elems=n) == -3
 
 
 def test_wrappers_refuse_before_they_reach_the_library():

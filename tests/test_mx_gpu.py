@@ -46,7 +46,7 @@ def depth(C):
     return max(64, C // 256) + 8 + 8
 
 
-WIDTHS = [1, 2, 7, 8, 31, 32, 33, 64, 200, 256, 384, 392, 768, 776, 1000, 1024, 1032, 1411, 2048, 2056, 2500, 4096, 4100, 4104, 8192, 8200]
+WIDTHS = [1, 2, 7, 8, 31, 32, 33, 64, 200, 256, 384, 392, 768, 776, 1000, 1024, 1032, 1411, 2048, 2056, 2500, 4096, 4100, 4104, 8192, 8200, 16384, 16390, 20001]
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
@@ -67,7 +67,7 @@ def test_norm_every_width(C, dtype, gpu_lib):
     same_bits(ops.rmsnorm(n["h"], w)["y"], ops.rmsnorm(n["h"].clone(), w)["y"])
 
 
-@pytest.mark.parametrize("C", [1, 31, 64, 200, 768, 1000, 1411, 2048, 4096, 4104, 8192, 8200])
+@pytest.mark.parametrize("C", [1, 31, 64, 200, 768, 1000, 1411, 2048, 4096, 4104, 8192, 8200, 16390])
 def test_norm_8_and_4_bits_are_the_quantised_norm(C, gpu_lib):
     """in fp32 the unrounded y is the output y: its e4m3 and MXFP4 forms are bit for bit what the quantisers make of it"""
     x, w = act(6, C, F32, C), 1 + 0.2 * torch.randn(C, generator=gen(C + 2)).cuda()
@@ -108,7 +108,7 @@ def test_norm_8_and_4_bits_of_bf16(rows, C, gpu_lib):
 
 def test_norm_in_place_strided_and_padded(gpu_lib):
     """h in x's or res's own memory, column slices of wider buffers (no 16-byte alignment), rows that stay as they were"""
-    for C in (768, 1411, 5000):
+    for C in (768, 1411, 5000, 17000):
         for dtype in (BF, F32):
             x, r, w = act(9, C, dtype, 3, wide=True), act(9, C, dtype, 4, wide=True), torch.rand(C, generator=gen(5)).cuda()
             want = ops.rmsnorm(x.contiguous(), w, res=r.contiguous())
@@ -133,7 +133,7 @@ def test_norm_in_place_strided_and_padded(gpu_lib):
 
 
 def test_norm_not_a_number_stays_in_its_row(gpu_lib):
-    for C in (768, 1411, 5000):
+    for C in (768, 1411, 5000, 17000):
         x, w = act(4, C, BF, 1), torch.ones(C, device="cuda")
         x[1, 5], x[2, 7] = float("nan"), float("inf")
         clean = act(4, C, BF, 1)
@@ -183,6 +183,14 @@ def test_norm_gradient_many_rows_and_none(gpu_lib):
         close(dw, wantw, (200 + rows // 256) * U * (d.double().cpu() * n).abs().sum(0), "dw")
         rel = float((dh.double().cpu() - want).norm() / want.norm())
         assert rel <= half(dt) + 1e-6
+        for own in (0, 1):                                                    # in place, where a workgroup has several rows and reads ahead
+            c = [h.clone(), d.clone()]
+            same_bits(ops.rmsnorm_bwd(c[0], rstd, c[1], w, dh=c[own])[0], dh)
+    wide, narrow = act(300, 1411, BF, 4, wide=True), act(300, 1411, BF, 4)     # strided and unaligned: the same sums in the same order
+    w = torch.rand(1411, generator=gen(3)).cuda()
+    rstd = mo.rms(narrow, w)[1].float().cuda()
+    for a, b in zip(ops.rmsnorm_bwd(wide, rstd, wide, w, dres=wide), ops.rmsnorm_bwd(narrow, rstd, narrow, w, dres=narrow)):
+        same_bits(a, b)
     h0 = torch.empty(0, 64, dtype=BF, device="cuda")
     dh, dw = ops.rmsnorm_bwd(h0, torch.empty(0, device="cuda"), h0, torch.ones(64, device="cuda"))
     assert dh.shape == (0, 64) and bool((dw == 0).all())
@@ -453,6 +461,22 @@ def test_layer_and_its_gradients_together(rows, C, N, gpu_lib):
     dW = ops.gemm_mxfp4(ops.quant_mxfp4(d, transpose=True), ops.quant_mxfp4(hb, transpose=True), out_dtype=F32)
     a, b = mo.values_of(*mo.codes_of(d.t())), mo.values_of(*mo.codes_of(hb.t()))
     close(dW, a @ b.t(), (a.shape[1] // 32 + 24) * U * (a.abs() @ b.abs().t()), "dW")
+
+
+def test_refusals_of_overlapping_buffers_and_mixed_places(gpu_lib):
+    x, w = act(4, 64, BF, 1), torch.ones(64, device="cuda")
+    with pytest.raises(L.DistError, match="different devices"):
+        ops.rmsnorm(x, torch.ones(64))
+    with pytest.raises(L.DistError, match="different devices"):
+        ops.gemm_mxfp4(operand(4, 64, 1)[0], tuple(t.cpu() for t in operand(8, 64, 1)[0]))
+    buf = torch.zeros(6, 64, dtype=BF, device="cuda")
+    for call in (lambda: ops.rmsnorm_bwd(buf[:4], torch.ones(4, device="cuda"), x, w, dh=buf[1:5]), lambda: ops.rmsnorm_bwd(x, torch.ones(4, device="cuda"), buf[:4].float(), w, dres=buf[:4], dh=buf[2:]),
+                 lambda: ops.gemm_mxfp4(operand(4, 64, 1)[0], operand(64, 64, 2)[0], res=buf[:4], out=buf[1:5])):
+        with pytest.raises(L.DistError, match="overlaps"):
+            call()
+    codes = torch.zeros(8, 64, dtype=torch.uint8, device="cuda")
+    with pytest.raises(L.DistError, match="overlaps"):
+        ops.gemm_mxfp4((codes, torch.zeros(1, 8, 8, dtype=torch.uint8, device="cuda")), operand(32, 128, 2)[0], out=codes.view(BF))
 
 
 def test_other_stream_and_two_graphs(gpu_lib):
