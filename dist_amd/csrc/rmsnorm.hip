@@ -253,14 +253,16 @@ __global__ __launch_bounds__(NT) void rms_bwd_kernel(const dist_rms_bwd_args p) 
             }
         }
     }
-    float* part = p.scratch + (long)blockIdx.x * C;
+    // the only workgroup (few rows) writes dw itself
+    const bool only = gridDim.x == 1, add = only && p.accumulate;
+    float* part = only ? p.dw : p.scratch + (long)blockIdx.x * C;
     if constexpr (LPR == NT) {
 #pragma unroll
         for (int it = 0; it < IT; ++it) {
             const int c = (lr + it * LPR) * 8;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (c + e < C) part[c + e] = aw[it][e];
+                if (c + e < C) part[c + e] = add ? part[c + e] + aw[it][e] : aw[it][e];
         }
     } else {
         for (int k = 0; k < RPB; ++k) {                                       // the block's row slots, one after the other
@@ -275,7 +277,7 @@ __global__ __launch_bounds__(NT) void rms_bwd_kernel(const dist_rms_bwd_args p) 
             }
             __syncthreads();
         }
-        for (int c = threadIdx.x; c < C; c += NT) part[c] = cols[c];
+        for (int c = threadIdx.x; c < C; c += NT) part[c] = add ? part[c] + cols[c] : cols[c];
     }
 }
 
@@ -331,7 +333,8 @@ constexpr int PARTIALS = 512;                                  // workgroups of 
 inline int bwd_lanes(int C) { return C <= 384 ? 16 : C <= 768 ? 32 : C <= 2048 ? 64 : C <= BWD_MAX ? 256 : 0; }
 inline int64_t bwd_partials(int64_t rows, int C) {
     const int lanes = bwd_lanes(C);
-    const int64_t need = lanes ? (rows + NT / lanes - 1) / (NT / lanes) : rows, most = lanes ? PARTIALS : 64;
+    const int64_t per = lanes ? NT / lanes : 1, need = (rows + per - 1) / per, most = lanes ? PARTIALS : 64;
+    if (lanes && need <= 4) return 1;                         // (few rows: a second launch costs more than a workgroup's four steps)
     return need < 1 ? 1 : need > most ? most : need;
 }
 inline bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
@@ -377,6 +380,7 @@ template <typename T, typename TD, bool AL> int bwd(const dist_rms_bwd_args& p, 
     else { if (p.C <= 4096) DIST_RMS(256, 2); else DIST_RMS(256, 4); }
 #undef DIST_RMS
     HIP_CHECK_RET(hipGetLastError());
+    if (lanes && G == 1) return DIST_OK;
     hipLaunchKernelGGL(rms_dw_kernel, dim3((unsigned)((p.C + 15) / 16)), dim3(1024), 0, s, p.scratch, G, p.C, p.dw, p.accumulate);
     HIP_CHECK_RET(hipGetLastError());
     return DIST_OK;

@@ -563,11 +563,11 @@ def _refuse(what):
 def _device(first, *others):
     """the index of the GPU that every operand is on"""
     dev = first.get_device()
-    if dev < 0:
-        _refuse("the operands must be GPU tensors")
     for t in others:
         if t is not None and t.get_device() != dev:
             _refuse(f"operands on different devices: {first.device} and {t.device}")
+    if dev < 0:
+        _refuse("the operands must be GPU tensors")
     return dev
 
 
@@ -780,7 +780,7 @@ def gemm_mxfp4(A, B, *, bias=None, res=None, out=None, out_dtype=torch.bfloat16)
         _vector(bias, N, "bias")
     ldres = _matrix(res, (M, N), "res", out.dtype) if res is not None else 0
     lib = L.load()
-    n = lib.dist_op_gemm_mxfp4_scratch(M, N, K, fmt)
+    n = lib.dist_op_gemm_mxfp4_scratch(M, N, K, fmt) if M > 64 else 0
     scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None
     a = L.GemmMxArgs(q.data_ptr(), sc.data_ptr(), B[0].data_ptr(), B[1].data_ptr(), bias.data_ptr() if bias is not None else None, res.data_ptr() if res is not None else None, out.data_ptr(),
                      scratch.data_ptr() if n > 0 else None, M, lda, ldc, ldres, n, N, K, fmt, dt)

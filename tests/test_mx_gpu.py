@@ -186,6 +186,12 @@ def test_norm_gradient_many_rows_and_none(gpu_lib):
         for own in (0, 1):                                                    # in place, where a workgroup has several rows and reads ahead
             c = [h.clone(), d.clone()]
             same_bits(ops.rmsnorm_bwd(c[0], rstd, c[1], w, dh=c[own])[0], dh)
+    for rows, C in ((1, 768), (4, 2048), (20, 300), (1, 8192), (8, 768), (33, 768)):          # one workgroup, and just more
+        h, d, w = act(rows, C, BF, 1), act(rows, C, BF, 2), torch.rand(C, generator=gen(3)).cuda()
+        rstd = mo.rms(h, w)[1].float().cuda()
+        dw = ops.rmsnorm_bwd(h, rstd, d, w, dw=torch.full((C,), 2.0, device="cuda"))[1]
+        n = h.double().cpu() * rstd.double().cpu()[:, None]
+        close(dw, (d.double().cpu() * n).sum(0) + 2, (rows + 24) * U * ((d.double().cpu() * n).abs().sum(0) + 2), "dw")
     wide, narrow = act(300, 1411, BF, 4, wide=True), act(300, 1411, BF, 4)     # strided and unaligned: the same sums in the same order
     w = torch.rand(1411, generator=gen(3)).cuda()
     rstd = mo.rms(narrow, w)[1].float().cuda()
