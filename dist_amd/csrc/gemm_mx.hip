@@ -125,93 +125,88 @@ struct Tile {
     static constexpr int W = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16;
     static constexpr int PA = A8 ? 128 : 64;                                       // bytes of a row of A in a stage
     static constexpr int A_BYTES = BM * PA, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES;
-    static constexpr int NA = A_BYTES / 1024, NB = B_BYTES / 1024, PER = (NA + NB) / W;     // DMA instructions of a stage, per wave
-    static constexpr int SA_BYTES = A8 ? 0 : (BM * 8 + 1023) / 1024 * 1024, SB_BYTES = (BN * 8 + 1023) / 1024 * 1024, SC = SA_BYTES + SB_BYTES;
-    static constexpr int NS = SC / 1024, PERS = (NS + W - 1) / W;                  // of the scales of 256 elements
+    static constexpr int NA = A_BYTES / 1024 / W, NB = B_BYTES / 1024 / W, PER = NA + NB;   // DMA instructions of a stage, per wave: of A, of B
+    static constexpr int NSA = A8 ? 0 : (BM * 8 + 1023) / 1024, NS = NSA + (BN * 8 + 1023) / 1024, SC = NS * 1024;      // of the scales of 256 elements, all waves
     static constexpr int LDS = S * STAGE + 2 * SC;
-    static_assert((NA + NB) % W == 0 && A_BYTES % 1024 == 0 && B_BYTES % 1024 == 0, "a stage is whole instructions for every wave");
+    static_assert(A_BYTES % (1024 * W) == 0 && B_BYTES % (1024 * W) == 0 && NS <= W, "whole instructions for every wave, at most one of scales");
+    static_assert(!A8 || NA % 2 == 0, "an e4m3 kilobyte is 8 rows, and the chunks' order repeats after 16");
 };
 
+// block -> tile: block b runs on XCD b % 8; every XCD takes a contiguous run of tiles, ordered in groups of 8 row tiles, so that the tiles an XCD works on at a time share row
+// and column panels in its L2.  `magic`: quotients by a whole group's tiles as a multiplication
+struct Grid { int ntm, ntn; unsigned magic; int shift; };
+inline Grid make_grid(long ntm, long ntn) {
+    Grid g{(int)ntm, (int)ntn, 0, 0};
+    const unsigned long d = 8 * ntn;                          // q = t / d for 0 <= t < 2^30: magic = ceil(2^(30 + shift) / d), 2^shift >= d
+    while ((1ul << g.shift) < d) ++g.shift;
+    g.magic = (unsigned)(((1ul << (30 + g.shift)) + d - 1) / d);
+    return g;
+}
+
 template <bool A8, bool RS, typename TO, int WM, int WN, int MT, int NT, int S, int OCC>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const dist_gemm_mx_args p, const int fast, const int ntm, const int ntn, const int slice) {
+__global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const dist_gemm_mx_args p, const Grid grid, const int fast, const int slice) {
     using T = Tile<A8, TO, WM, WN, MT, NT, S>;
     extern __shared__ char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const int wm = wave / WN, wn = wave % WN;
-    // block -> tile: block b runs on XCD b % 8; every XCD takes a contiguous run of tiles, ordered in groups of 8 row tiles, so that the tiles an XCD works on at a time
-    // share row and column panels in its L2
-    const int total = ntm * ntn, part = blockIdx.x / total, block = blockIdx.x - part * total, xcd = block & 7, each = total >> 3, more = total & 7;
-    const int t0 = xcd * each + min(xcd, more) + (block >> 3);
-    const int grp = t0 / (8 * ntn), in = t0 - grp * 8 * ntn, gm = min(8, ntm - grp * 8);
-    const long m0 = (long)(grp * 8 + in % gm) * T::BM;
-    const int n0 = (in / gm) * T::BN;
+    const int part = blockIdx.y, xcd = blockIdx.x & 7, each = gridDim.x >> 3, more = gridDim.x & 7;
+    const int t0 = xcd * each + min(xcd, more) + (int)(blockIdx.x >> 3);
+    const int grp = (int)(((unsigned long)(unsigned)t0 * grid.magic) >> (30 + grid.shift)), in = t0 - grp * 8 * grid.ntn, gm = grid.ntm - grp * 8;
+    const int tn = gm >= 8 ? in >> 3 : in / gm, tm = grp * 8 + (gm >= 8 ? in & 7 : in - tn * gm);
+    const long m0 = (long)tm * T::BM;
+    const int n0 = tn * T::BN;
 
     // elements k0 ... k0 + K of the long axis: all of them, or slice number `part` (then C is its fp32 partial result, without bias, residual and row scales)
     const int k0 = part * slice, K = min(slice, p.K - k0), chunk0 = k0 >> 8;
-    const long pitch_a = A8 ? p.lda : p.K / 2, pitch_b = p.K / 2;
+    const int pitch_a = A8 ? (int)p.lda : p.K / 2, pitch_b = p.K / 2;
     const int mrows = (int)min((long)T::BM, p.M - m0), nrows = min(T::BN, p.N - n0), ka = A8 ? k0 : k0 / 2;
-    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.A) + m0 * pitch_a + ka), 0, (int)(mrows * pitch_a - ka), 0x00020000);
-    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.B) + n0 * pitch_b + k0 / 2), 0, (int)(nrows * pitch_b - k0 / 2), 0x00020000);
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.A) + m0 * pitch_a + ka), 0, mrows * pitch_a - ka, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.B) + (long)n0 * pitch_b + k0 / 2), 0, nrows * pitch_b - k0 / 2, 0x00020000);
     const int nk = (K + 127) / 128, tail = K - (nk - 1) * 128;                     // stages; elements of the last one
 
-    // this wave's kilobytes of a stage: which operand, and the lane's offset in it
-    unsigned voff[T::PER];
-    int vchunk[T::PER];                                                            // first element of the lane's 16 bytes inside the stage
+    // The lane's offsets: its row of the wave's first kilobyte and its chunk; the further kilobytes are steps of whole rows in the scalar offset, which the descriptor's range
+    // check counts in.  (Registers of their own that change once, under a branch: hipcc waits for every load in flight before it reuses one that a load takes its address from.)
+    constexpr int LPR = T::PA / 16, RPK = 64 / LPR, VA = A8 ? 2 : 1;               // lanes per row of A, rows of a kilobyte, kinds of kilobytes
+    unsigned va[VA], vb;
+    auto offsets = [&](const int limit) __attribute__((always_inline)) {           // limit: elements of the stage, what lies behind is sent away
 #pragma unroll
-    for (int q = 0; q < T::PER; ++q) {
-        const int k = wave * T::PER + q;
-        constexpr int LPR = T::PA / 16;                                            // lanes per row of A
-        const bool isa = k < T::NA;
-        const int r = isa ? k * (64 / LPR) + lane / LPR : (k - T::NA) * 16 + (lane >> 2);
-        const int c = isa ? (lane % LPR) ^ a_swz<A8>(r) : (lane & 3) ^ b_swz<TO>(r);
-        voff[q] = (unsigned)(r * (isa ? pitch_a : pitch_b)) + c * 16;
-        vchunk[q] = c * (isa && A8 ? 16 : 32);
-    }
+        for (int q = 0; q < VA; ++q) {
+            const int r = wave * T::NA * RPK + lane / LPR, c = (lane % LPR) ^ a_swz<A8>(r + q * RPK);
+            va[q] = c * (A8 ? 16 : 32) >= limit ? FAR_AWAY : (unsigned)(r * pitch_a + c * 16);
+            regs_pin(va[q]);
+        }
+        const int r = wave * T::NB * 16 + (lane >> 2), c = (lane & 3) ^ b_swz<TO>(r);
+        vb = c * 32 >= limit ? FAR_AWAY : (unsigned)(r * pitch_b + c * 16);
+        regs_pin(vb);
+    };
+    offsets(128);
     auto issue = [&](const int kt) __attribute__((always_inline)) {
         char* base = smem + (kt % S) * T::STAGE;
-        // (the offsets live in the same registers for the whole loop and change once, under a branch: hipcc waits for every load in flight before it reuses a register that
-        // one of them takes its address from)
-        if (kt == nk - 1 && tail < 128) {
+        if (kt == nk - 1 && tail < 128) offsets(tail);
 #pragma unroll
-            for (int q = 0; q < T::PER; ++q) {
-                if (vchunk[q] >= tail) voff[q] = FAR_AWAY;
-                regs_pin(voff[q]);
-            }
+        for (int q = 0; q < T::NA; ++q) {
+            const unsigned v = va[q % VA];
+            const int step = kt * T::PA + q * RPK * pitch_a;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr)(base + (wave * T::NA + q) * 1024), 16, v, step, 0, 0);
         }
 #pragma unroll
-        for (int q = 0; q < T::PER; ++q) {
-            const int k = wave * T::PER + q;                                       // wave-uniform
-            const bool isa = k < T::NA;
-            const unsigned v = voff[q];
-            const int step = kt * (isa ? T::PA : 64);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(isa ? ra : rb, (lds_ptr)(base + k * 1024), 16, v, step, 0, 0);
+        for (int q = 0; q < T::NB; ++q) {
+            const unsigned v = vb;
+            const int step = kt * 64 + q * 16 * pitch_b;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr)(base + T::A_BYTES + (wave * T::NB + q) * 1024), 16, v, step, 0, 0);
         }
     };
-    // the scales' kilobytes of this wave: source, what is there to read and the step to the next 256 elements (a wave without one of its own repeats the last: the
-    // same bytes to the same place)
-    const char* ssrc[T::PERS];
-    long sstep[T::PERS];
-    int sleft[T::PERS], sdst[T::PERS];
-#pragma unroll
-    for (int q = 0; q < T::PERS; ++q) {
-        const int k = min(wave * T::PERS + q, T::NS - 1);
-        sdst[q] = S * T::STAGE + k * 1024;
-        if (k < T::SA_BYTES / 1024) {
-            ssrc[q] = static_cast<const char*>(p.a_scale) + ((long)chunk0 * p.M + m0) * 8 + k * 1024;
-            sstep[q] = p.M * 8;
-            sleft[q] = max(mrows * 8 - k * 1024, 0);
-        } else {
-            ssrc[q] = static_cast<const char*>(p.b_scale) + ((long)chunk0 * p.N + n0) * 8 + (k * 1024 - T::SA_BYTES);
-            sstep[q] = (long)p.N * 8;
-            sleft[q] = max(nrows * 8 - (k * 1024 - T::SA_BYTES), 0);
-        }
-    }
+    // the wave's kilobyte of scales (a wave without one of its own repeats the last: the same bytes to the same place)
+    const int sk = min(wave, T::NS - 1);
+    const bool sa = sk < T::NSA;
+    const long sstep = (sa ? p.M : (long)p.N) * 8;
+    const int sfirst = (sa ? sk : sk - T::NSA) * 1024, sleft = max((sa ? mrows : nrows) * 8 - sfirst, 0);
+    const char* const ssrc = (sa ? static_cast<const char*>(p.a_scale) + m0 * 8 : static_cast<const char*>(p.b_scale) + (long)n0 * 8) + chunk0 * sstep + sfirst;
+    unsigned lane16 = lane * 16;
+    regs_pin(lane16);
     auto issue_scales = [&](const int chunk) __attribute__((always_inline)) {
-#pragma unroll
-        for (int q = 0; q < T::PERS; ++q) {
-            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(ssrc[q] + chunk * sstep[q]), 0, sleft[q], 0x00020000);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(smem + sdst[q] + (chunk & 1) * T::SC), 16, lane * 16, 0, 0, 0);
-        }
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(ssrc + chunk * sstep), 0, sleft, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(smem + S * T::STAGE + sk * 1024 + (chunk & 1) * T::SC), 16, lane16, 0, 0, 0);
     };
 
     // LDS addresses of this lane's fragments inside a stage
@@ -231,7 +226,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const d
     auto stage = [&](auto par, const int kt) __attribute__((always_inline)) {
         constexpr int P = decltype(par)::value;                                    // kt & 1: which byte of the scales
         // stages kt + 1 ... kt + S - 2 may stay in flight; of two neighbours one carries scales
-        if (kt + S - 2 < nk) wait_vm<(S - 2) * T::PER + ((S - 2 + (P ? 1 : 0)) / 2) * T::PERS>();
+        if (kt + S - 2 < nk) wait_vm<(S - 2) * T::PER + ((S - 2 + (P ? 1 : 0)) / 2)>();
         else wait_vm<0>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
@@ -247,7 +242,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const d
 #pragma unroll
                 for (int t = 0; t < MT; ++t) as[t] = *reinterpret_cast<const unsigned short*>(sc + (arow + t * 16) * 8 + 2 * g);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) bs[j] = *reinterpret_cast<const unsigned short*>(sc + T::SA_BYTES + (brow + frag_col<TO>(j)) * 8 + 2 * g);
+            for (int j = 0; j < NT; ++j) bs[j] = *reinterpret_cast<const unsigned short*>(sc + T::NSA * 1024 + (brow + frag_col<TO>(j)) * 8 + 2 * g);
         }
         v8i_t a[MT], b[NT];
 #pragma unroll
@@ -288,18 +283,17 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const d
         const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(C) + (m0 * p.ldc + n0) * ES, 0, (int)((mrows * p.ldc - n0) * ES), 0x00020000);
         const __amdgpu_buffer_rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.res)) + (m0 * p.ldres + n0) * ES, 0, p.res ? (int)((mrows * p.ldres - n0) * ES) : 0, 0x00020000);
         const bool up = (i & 8) != 0;
-        const int rowx = rowl - (up ? 8 : 0);
+        const int colx = coll + (up ? frag_col<TO>(U) : 0), stepc = (int)(8 * p.ldc * ES), stepr = (int)(16 * p.ldres * ES);
+        const unsigned cbase = (unsigned)((rowl - (up ? 8 : 0)) * (int)p.ldc + colx) * ES, rbase = (unsigned)(rowl * (int)p.ldres + coll) * ES;
 #pragma unroll
         for (int j = 0; j < NT; j += 2 * U) {
-            const int col = coll + frag_col<TO>(j) + (up ? frag_col<TO>(U) : 0);
-            const bool in = n0 + col < p.N;
             v4u_t q[MT][2];
             if (p.res) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    const unsigned o = (unsigned)(((rowx + t * 16) * p.ldres + col) * ES);
-                    q[t][0] = __builtin_amdgcn_raw_buffer_load_b128(rr, in ? o : FAR_AWAY, 0, 0);
-                    q[t][1] = __builtin_amdgcn_raw_buffer_load_b128(rr, in ? o + (unsigned)(8 * p.ldres * ES) : FAR_AWAY, 0, 0);
+                for (int h = 0; h < 2; ++h) {
+                    const unsigned v = n0 + coll + frag_col<TO>(j + h * U) < p.N ? rbase + frag_col<TO>(j + h * U) * ES : FAR_AWAY;
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) q[t][h] = __builtin_amdgcn_raw_buffer_load_b128(rr, v, t * stepr, 0);
                 }
             }
             float bias[2][4 * U];
@@ -313,51 +307,41 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const d
                     else load4(p.bias + n, bias[h]);
                 }
             }
+            const unsigned at = n0 + colx + frag_col<TO>(j) < p.N ? cbase + frag_col<TO>(j) * ES : FAR_AWAY;
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                float own[2][4 * U];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 4 * U; ++e) own[h][e] = (A8 ? acc[t][j + h * U + e / 4][e % 4] * rs[t] : acc[t][j + h * U + e / 4][e % 4]) + bias[h][e];
-                if (p.res) {                                                       // in fp32: exchange, add, round
-#pragma unroll
-                    for (int e = 0; e < 4 * U; ++e) {
-                        const float got = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(up ? own[0][e] : own[1][e]), 0x128 /* row_ror:8 */, 0xf, 0xf, true));
-                        if (up) own[0][e] = got; else own[1][e] = got;
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if constexpr (U == 2) {
-                            const bf16x8 f = __builtin_bit_cast(bf16x8, q[t][h]);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) own[h][e] += (float)f[e];
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) own[h][e] += __uint_as_float(q[t][h][e]);
-                        }
-                    }
-                }
                 v4u_t out[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
+                    float v[4 * U];
+#pragma unroll
+                    for (int e = 0; e < 4 * U; ++e) v[e] = (A8 ? acc[t][j + h * U + e / 4][e % 4] * rs[t] : acc[t][j + h * U + e / 4][e % 4]) + bias[h][e];
                     if constexpr (U == 2) {
+                        if (p.res) {
+                            const bf16x8 f = __builtin_bit_cast(bf16x8, q[t][h]);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] += (float)f[e];
+                        }
                         Frag<bf16_t> f;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) frag_set(f, e, own[h][e]);
+                        for (int e = 0; e < 8; ++e) frag_set(f, e, v[e]);
                         out[h] = __builtin_bit_cast(v4u_t, f.v);
-                    } else out[h] = v4u_t{__float_as_uint(own[h][0]), __float_as_uint(own[h][1]), __float_as_uint(own[h][2]), __float_as_uint(own[h][3])};
-                }
-                if (!p.res) {
+                    } else {
+                        if (p.res) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const unsigned got = __builtin_amdgcn_update_dpp(0, (int)(up ? out[0][e] : out[1][e]), 0x128, 0xf, 0xf, true);
-                        if (up) out[0][e] = got; else out[1][e] = got;
+                            for (int e = 0; e < 4; ++e) v[e] += __uint_as_float(q[t][h][e]);
+                        }
+                        out[h] = v4u_t{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
                     }
                 }
-                const unsigned o = (unsigned)(((rowx + t * 16) * p.ldc + col) * ES);
-                __builtin_amdgcn_raw_buffer_store_b128(out[0], rc, in ? o : FAR_AWAY, 0, 2);
-                __builtin_amdgcn_raw_buffer_store_b128(out[1], rc, in ? o + (unsigned)(8 * p.ldc * ES) : FAR_AWAY, 0, 2);
+                v4u_t o0, o1;                                                      // rows 0 ... 7: the upper lanes take the lower lanes' second half;  rows 8 ... 15 the other way
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    o0[e] = (unsigned)__builtin_amdgcn_update_dpp((int)out[0][e], (int)out[1][e], 0x128 /* row_ror:8 */, 0xf, 0xc, false);
+                    o1[e] = (unsigned)__builtin_amdgcn_update_dpp((int)out[1][e], (int)out[0][e], 0x128, 0xf, 0x3, false);
+                }
+                __builtin_amdgcn_raw_buffer_store_b128(o0, rc, at, 2 * t * stepc, 2);
+                __builtin_amdgcn_raw_buffer_store_b128(o1, rc, at, (2 * t + 1) * stepc, 2);
             }
         }
         return;
@@ -393,14 +377,14 @@ __global__ __launch_bounds__(NT_) void gemm_mx_join_kernel(const dist_gemm_mx_ar
 template <bool A8, bool RS, typename TO, int WM, int WN, int MT, int NT, int S, int OCC> int launch_tile(const dist_gemm_mx_args& p, int slice, hipStream_t s) {
     using T = Tile<A8, TO, WM, WN, MT, NT, S>;
     const long ntm = (p.M + T::BM - 1) / T::BM, ntn = (p.N + T::BN - 1) / T::BN, parts = (p.K + slice - 1) / slice;
-    if (ntm * ntn * parts > 0x3fffffff) return DIST_ERR_ARG;
+    if (ntm * ntn >= 1 << 30 || parts > 65535) return DIST_ERR_ARG;
     const auto k = gemm_mx_tile_kernel<A8, RS, TO, WM, WN, MT, NT, S, OCC>;
     static DistSmemOnce st;
     RUN_(dist_max_smem(st, reinterpret_cast<const void*>(k), T::LDS));
     constexpr size_t ES = sizeof(TO);
     const bool fast = p.N % (16 / ES) == 0 && (uintptr_t)p.C % 16 == 0 && p.ldc * ES % 16 == 0 && p.ldc <= 1 << 20 && (!p.bias || (uintptr_t)p.bias % 16 == 0) &&
                       (!p.res || ((uintptr_t)p.res % 16 == 0 && p.ldres * ES % 16 == 0 && p.ldres <= 1 << 20));
-    hipLaunchKernelGGL(k, dim3((unsigned)(ntm * ntn * parts)), dim3(64 * T::W), T::LDS, s, p, (int)fast, (int)ntm, (int)ntn, slice);
+    hipLaunchKernelGGL(k, dim3((unsigned)(ntm * ntn), (unsigned)parts), dim3(64 * T::W), T::LDS, s, p, make_grid(ntm, ntn), (int)fast, slice);
     HIP_CHECK_RET(hipGetLastError());
     return DIST_OK;
 }
