@@ -276,6 +276,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const d
     for (int t = 0; t < MT; ++t) rs[t] = A8 && RS && mw + t * 16 < p.M ? static_cast<const float*>(p.a_scale)[mw + t * 16] : 1.f;
     // 16-byte stores through a descriptor that ends behind the last row; columns behind N are sent past it.  Lanes i and i ^ 8 exchange, so that a store writes 8 rows of
     // 128 bytes and not 16 of 64, past the caches' keeping: a 232 MB output takes 43 us this way and 64 us in half lines kept in the L2
+    // (The steps of the rows are in the lanes' offset: behind a 16-byte store whose scalar offset is a register hipcc writes the store's data anew in the very next instruction,
+    // and gfx950 then stores the new value in some lanes.  With a constant scalar offset hipcc keeps the distance.)
     constexpr int U = sizeof(TO) == 2 ? 2 : 1, ES = sizeof(TO);                    // fragments of one 16-byte store
     const int rowl = wm * MT * 16 + i, coll = wn * NT * 16 + g * (4 * U);
     TO* const C = static_cast<TO*>(p.C) + part * (p.M * p.ldc);                    // (slices lie one behind the other)
@@ -340,8 +342,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const d
                     o0[e] = (unsigned)__builtin_amdgcn_update_dpp((int)out[0][e], (int)out[1][e], 0x128 /* row_ror:8 */, 0xf, 0xc, false);
                     o1[e] = (unsigned)__builtin_amdgcn_update_dpp((int)out[1][e], (int)out[0][e], 0x128, 0xf, 0x3, false);
                 }
-                __builtin_amdgcn_raw_buffer_store_b128(o0, rc, at, 2 * t * stepc, 2);
-                __builtin_amdgcn_raw_buffer_store_b128(o1, rc, at, (2 * t + 1) * stepc, 2);
+                __builtin_amdgcn_raw_buffer_store_b128(o0, rc, at + 2 * t * stepc, 0, 2);
+                __builtin_amdgcn_raw_buffer_store_b128(o1, rc, at + (2 * t + 1) * stepc, 0, 2);
             }
         }
         return;

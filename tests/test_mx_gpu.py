@@ -346,6 +346,29 @@ def test_product_sizes_of_use(M, N, K, fmt, out, gpu_lib):
     check_product(M, N, K, fmt, out, True, True, 5)
 
 
+@pytest.mark.parametrize("M,N,K,fmt,out", [(2600, 2304, 768, "mxfp4", BF), (2600, 2304, 768, "e4m3", BF), (4096, 2304, 768, "mxfp4", F32), (2600, 2304, 1024, "mxfp4", BF), (12608, 2304, 768, "mxfp4", BF),
+                                           (300, 520, 2048, "mxfp4", F32), (300, 520, 2048, "e4m3", BF)])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("res", [False, True])
+def test_product_same_bits_every_time(M, N, K, fmt, out, bias, res, gpu_lib):
+    # every epilogue, many calls: a store whose data is written anew too early differs from call to call
+    B, b = operand(N, K, 1)
+    A, a = operand(M, K, 2) if fmt == "mxfp4" else rows8(M, K, 2)
+    bi = torch.randn(N, generator=gen(3)).cuda() if bias else None
+    r = torch.randn(M, N, generator=gen(4)).to(out).cuda() if res else None
+    first = ops.gemm_mxfp4(A, B, bias=bi, res=r, out_dtype=out)
+    a, b = a.float().cuda(), b.float().cuda()
+    want, mag = a @ b.t(), a.abs() @ b.abs().t()
+    for t in (bi, r):
+        if t is not None:
+            want, mag = want + t.float(), mag + t.float().abs()
+    # (the comparison sums K products in fp32 itself)
+    tol = 2 * (K + 16) * U * mag + half(out) * want.abs() + (2.0 ** -10 * mag if fmt == "e4m3" else 0)
+    assert bool(((first.float() - want).abs() <= tol).all())
+    for _ in range(20):
+        same_bits(first, ops.gemm_mxfp4(A, B, bias=bi, res=r, out_dtype=out))
+
+
 def test_product_into_buffers(gpu_lib):
     """out and res as columns of wider buffers, at any alignment; rows behind the last one and columns beside it stay as they were; res in out's own memory"""
     for M, N, K in ((5, 64, 96), (70, 129, 288), (300, 256, 256)):
