@@ -96,15 +96,16 @@ __global__ __launch_bounds__(64 * W) void gemm_mx_few_kernel(const dist_gemm_mx_
 }
 
 // ---- tiles through LDS ------------------------------------------------------------------------------------------------------------------------------------------
-// WM x WN waves, each a 16 MT x 16 NT tile of outputs.  K advances by 128 elements a stage (one instruction deep): rows of 64 bytes of codes (e4m3: 128 bytes) go to LDS by
-// LDS-DMA into a ring of S stages, S - 1 of them in flight; one barrier per stage, behind a counted wait: when it opens, stage t has landed for every wave and stage
-// t - 1 is read by nobody, so its place receives stage t + S - 1.  Scale bytes follow per 256 elements into a ring of their own, with the stage that needs them first.
-// A 16-byte chunk c of row r lies at chunk c ^ f(r), applied where the DMA reads (its LDS side is lane-linear).  Descriptors end behind the last row, and chunks behind K are
-// sent past the end: all of these read as zeros.
-// Measured (50432 x 2304 x 768, 4-bit operands, bf16 out): 95 us = 1.9 PF, of it 55 us when nothing is stored and 43 us when only the outputs are (5.4 TB/s): with six
-// stages a tile the workgroups of a CU stay in step, and the two add up.  Deep (16448 x 1024 x 4096, e4m3): 78 us = 1.8 PF, by the 41 GB/s a CU draws through its LDS-DMA.
-// Built and not faster: workgroups that stay and prefetch across tiles (88 - 91 and 97 us), fragments read half a stage ahead (no change), three or four stages in the ring,
-// all reads in front of the matrix instructions, raised priority around them (all within 3 %).
+// WM x WN waves, each a 16 MT x 16 NT tile of outputs.  K advances by 256 elements a stage (4-bit operands: two instructions deep) or 128 (e4m3): rows of 128 bytes of A and
+// of 64 D bytes of B go to LDS by LDS-DMA into a ring of S stages, S - 1 of them in flight; one barrier per stage, behind a counted wait: when it opens, stage t has landed for
+// every wave and stage t - 1 is read by nobody, so its place receives stage t + S - 1.  Scale bytes follow per 256 elements into a ring of their own, with the stage that needs
+// them first.  A 16-byte chunk c of row r lies at chunk c ^ f(r), applied where the DMA reads (its LDS side is lane-linear).  Descriptors end behind the last row, and chunks
+// behind K are sent past the end: all of these read as zeros.
+// Measured (50432 x 2304 x 768, 4-bit operands, bf16 out): 83 us = 2.15 PF (stages of 128 elements: 95); of it 43 us are the outputs' stores (5.4 TB/s), which with three
+// stages a tile add to the loop more than they hide behind it.  4096^3: 39 us = 3.5 PF.  Deep (16448 x 1024 x 4096, e4m3): 78 us = 1.8 PF, by the 41 GB/s a CU draws through
+// its LDS-DMA.
+// Built and not faster (in stages of 128): workgroups that stay and prefetch across tiles, fragments read half a stage ahead, three or four stages in the ring, all reads in
+// front of the matrix instructions, raised priority around them (all within 5 %).
 typedef __attribute__((address_space(3))) void* lds_ptr;
 DEV void regs_pin(unsigned& v) { asm volatile("" : "+v"(v)); }
 template <int N> DEV void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
@@ -117,19 +118,19 @@ template <typename TO> DEV int lane_col(int i) { return sizeof(TO) == 2 ? (i >> 
 
 // (8 lanes read 128 bytes at a time: their 8 rows - consecutive ones of A, 0 ... 3 and 8 ... 11 of a 16-bit B - must fall on different 16-byte places.  ds_read_b128 then
 // moves 234 bytes a clock and CU; patterns that are free of conflicts over 16 lanes only reach 127.)
-template <bool A8> DEV int a_swz(int r) { return A8 ? (r >> 1) & 7 : (r >> 1) & 3; }
+DEV int a_swz(int r) { return (r >> 1) & 7; }
 template <typename TO> DEV int b_swz(int r) { return sizeof(TO) == 2 ? ((r >> 1) & 1) | ((r >> 2) & 2) : (r >> 1) & 3; }
 
 template <bool A8, typename TO, int WM, int WN, int MT, int NT, int S>
 struct Tile {
     static constexpr int W = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16;
-    static constexpr int PA = A8 ? 128 : 64;                                       // bytes of a row of A in a stage
-    static constexpr int A_BYTES = BM * PA, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES;
+    static constexpr int D = A8 ? 1 : 2, PB = 64 * D;                              // instructions along K in a stage; bytes of a row of B in it (of A: 128)
+    static constexpr int A_BYTES = BM * 128, B_BYTES = BN * PB, STAGE = A_BYTES + B_BYTES;
     static constexpr int NA = A_BYTES / 1024 / W, NB = B_BYTES / 1024 / W, PER = NA + NB;   // DMA instructions of a stage, per wave: of A, of B
     static constexpr int NSA = A8 ? 0 : (BM * 8 + 1023) / 1024, NS = NSA + (BN * 8 + 1023) / 1024, SC = NS * 1024;      // of the scales of 256 elements, all waves
-    static constexpr int LDS = S * STAGE + 2 * SC;
+    static constexpr int SCN = A8 ? 2 : S, LDS = S * STAGE + SCN * SC;       // places in the scales' ring
     static_assert(A_BYTES % (1024 * W) == 0 && B_BYTES % (1024 * W) == 0 && NS <= W, "whole instructions for every wave, at most one of scales");
-    static_assert(!A8 || NA % 2 == 0, "an e4m3 kilobyte is 8 rows, and the chunks' order repeats after 16");
+    static_assert(NA % 2 == 0 && (D == 1 || NB % 2 == 0), "a kilobyte of 128-byte rows is 8 of them, and the chunks' order repeats after 16");
 };
 
 // block -> tile: block b runs on XCD b % 8; every XCD takes a contiguous run of tiles, ordered in groups of 8 row tiles, so that the tiles an XCD works on at a time share row
@@ -162,40 +163,28 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const d
     const int mrows = (int)min((long)T::BM, p.M - m0), nrows = min(T::BN, p.N - n0), ka = A8 ? k0 : k0 / 2;
     const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.A) + m0 * pitch_a + ka), 0, mrows * pitch_a - ka, 0x00020000);
     const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.B) + (long)n0 * pitch_b + k0 / 2), 0, nrows * pitch_b - k0 / 2, 0x00020000);
-    const int nk = (K + 127) / 128, tail = K - (nk - 1) * 128;                     // stages; elements of the last one
+    constexpr int KS = 128 * T::D;
+    const int nk = (K + KS - 1) / KS, tail = K - (nk - 1) * KS;                     // stages; elements of the last one
 
     // The lane's offsets: its row of the wave's first kilobyte and its chunk; the further kilobytes are steps of whole rows in the scalar offset, which the descriptor's range
     // check counts in.  (Registers of their own that change once, under a branch: hipcc waits for every load in flight before it reuses one that a load takes its address from.)
-    constexpr int LPR = T::PA / 16, RPK = 64 / LPR, VA = A8 ? 2 : 1;               // lanes per row of A, rows of a kilobyte, kinds of kilobytes
-    unsigned va[VA], vb;
+    constexpr int LB = T::PB / 16, RB = 64 / LB;                                   // lanes per row of B, rows of a kilobyte (of A: 8 and 8)
+    unsigned va[2], vb[T::D];                                                      // (the chunks' order repeats after 16 rows)
     auto offsets = [&](const int limit) __attribute__((always_inline)) {           // limit: elements of the stage, what lies behind is sent away
 #pragma unroll
-        for (int q = 0; q < VA; ++q) {
-            const int r = wave * T::NA * RPK + lane / LPR, c = (lane % LPR) ^ a_swz<A8>(r + q * RPK);
+        for (int q = 0; q < 2; ++q) {
+            const int r = wave * T::NA * 8 + (lane >> 3), c = (lane & 7) ^ a_swz(r + q * 8);
             va[q] = c * (A8 ? 16 : 32) >= limit ? FAR_AWAY : (unsigned)(r * pitch_a + c * 16);
             regs_pin(va[q]);
         }
-        const int r = wave * T::NB * 16 + (lane >> 2), c = (lane & 3) ^ b_swz<TO>(r);
-        vb = c * 32 >= limit ? FAR_AWAY : (unsigned)(r * pitch_b + c * 16);
-        regs_pin(vb);
-    };
-    offsets(128);
-    auto issue = [&](const int kt) __attribute__((always_inline)) {
-        char* base = smem + (kt % S) * T::STAGE;
-        if (kt == nk - 1 && tail < 128) offsets(tail);
 #pragma unroll
-        for (int q = 0; q < T::NA; ++q) {
-            const unsigned v = va[q % VA];
-            const int step = kt * T::PA + q * RPK * pitch_a;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr)(base + (wave * T::NA + q) * 1024), 16, v, step, 0, 0);
-        }
-#pragma unroll
-        for (int q = 0; q < T::NB; ++q) {
-            const unsigned v = vb;
-            const int step = kt * 64 + q * 16 * pitch_b;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr)(base + T::A_BYTES + (wave * T::NB + q) * 1024), 16, v, step, 0, 0);
+        for (int q = 0; q < T::D; ++q) {
+            const int r = wave * T::NB * RB + lane / LB, c = (lane % LB) ^ b_swz<TO>(r + q * RB);
+            vb[q] = c * 32 >= limit ? FAR_AWAY : (unsigned)(r * pitch_b + c * 16);
+            regs_pin(vb[q]);
         }
     };
+    offsets(KS);
     // the wave's kilobyte of scales (a wave without one of its own repeats the last: the same bytes to the same place)
     const int sk = min(wave, T::NS - 1);
     const bool sa = sk < T::NSA;
@@ -206,13 +195,31 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const d
     regs_pin(lane16);
     auto issue_scales = [&](const int chunk) __attribute__((always_inline)) {
         const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(ssrc + chunk * sstep), 0, sleft, 0x00020000);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(smem + S * T::STAGE + sk * 1024 + (chunk & 1) * T::SC), 16, lane16, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(smem + S * T::STAGE + sk * 1024 + (chunk % T::SCN) * T::SC), 16, lane16, 0, 0, 0);
+    };
+    auto issue = [&](const int kt) __attribute__((always_inline)) {
+        char* base = smem + (kt % S) * T::STAGE;
+        if (!A8) issue_scales(kt);
+        else if ((kt & 1) == 0) issue_scales(kt >> 1);
+        if (kt == nk - 1 && tail < KS) offsets(tail);
+#pragma unroll
+        for (int q = 0; q < T::NA; ++q) {
+            const unsigned v = va[q % 2];
+            const int step = kt * 128 + q * 8 * pitch_a;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr)(base + (wave * T::NA + q) * 1024), 16, v, step, 0, 0);
+        }
+#pragma unroll
+        for (int q = 0; q < T::NB; ++q) {
+            const unsigned v = vb[q % T::D];
+            const int step = kt * T::PB + q * RB * pitch_b;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr)(base + T::A_BYTES + (wave * T::NB + q) * 1024), 16, v, step, 0, 0);
+        }
     };
 
     // LDS addresses of this lane's fragments inside a stage
     const int arow = wm * MT * 16 + i, brow = wn * NT * 16 + lane_col<TO>(i);
-    const int a_lo = arow * T::PA + ((g ^ a_swz<A8>(arow)) << 4), a_hi = arow * T::PA + (((4 + g) ^ a_swz<A8>(arow)) << 4);
-    const int b_at = T::A_BYTES + brow * 64 + ((g ^ b_swz<TO>(brow)) << 4);
+    const int a_lo = arow * 128 + ((g ^ a_swz(arow)) << 4), a_hi = arow * 128 + (((4 + g) ^ a_swz(arow)) << 4);
+    const int b_lo = T::A_BYTES + brow * T::PB + ((g ^ b_swz<TO>(brow)) << 4), b_hi = T::A_BYTES + brow * T::PB + (((4 + g) ^ b_swz<TO>(brow)) << 4);
 
     f32x4 acc[MT][NT];
 #pragma unroll
@@ -223,50 +230,55 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_mx_tile_kernel(const d
 #pragma unroll
     for (int t = 0; t < MT; ++t) as[t] = 127;
 
+    // stage kt; P: which half of 256 elements it begins with (e4m3: kt & 1, 4-bit operands: 0)
     auto stage = [&](auto par, const int kt) __attribute__((always_inline)) {
-        constexpr int P = decltype(par)::value;                                    // kt & 1: which byte of the scales
-        // stages kt + 1 ... kt + S - 2 may stay in flight; of two neighbours one carries scales
-        if (kt + S - 2 < nk) wait_vm<(S - 2) * T::PER + ((S - 2 + (P ? 1 : 0)) / 2)>();
+        constexpr int P = decltype(par)::value, SCALES = A8 ? (S - 2 + P) / 2 : S - 2;     // kilobytes of scales among stages kt + 1 ... kt + S - 2, which may stay in flight
+        if (kt + S - 2 < nk) wait_vm<(S - 2) * T::PER + SCALES>();
         else wait_vm<0>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        if (kt + S - 1 < nk) {
-            if (((kt + S - 1) & 1) == 0) issue_scales((kt + S - 1) >> 1);
-            issue(kt + S - 1);
-        }
+        if (kt + S - 1 < nk) issue(kt + S - 1);
         __builtin_amdgcn_sched_barrier(0);
         const char* base = smem + (kt % S) * T::STAGE;
         if constexpr (P == 0) {
-            const char* sc = smem + S * T::STAGE + ((kt >> 1) & 1) * T::SC;
+            const char* sc = smem + S * T::STAGE + ((A8 ? kt >> 1 : kt) % T::SCN) * T::SC;
             if constexpr (!A8)
 #pragma unroll
                 for (int t = 0; t < MT; ++t) as[t] = *reinterpret_cast<const unsigned short*>(sc + (arow + t * 16) * 8 + 2 * g);
 #pragma unroll
             for (int j = 0; j < NT; ++j) bs[j] = *reinterpret_cast<const unsigned short*>(sc + T::NSA * 1024 + (brow + frag_col<TO>(j)) * 8 + 2 * g);
         }
-        v8i_t a[MT], b[NT];
+        auto step = [&](auto half) __attribute__((always_inline)) {
+            constexpr int H = decltype(half)::value;
+            v8i_t a[MT], b[NT];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            if constexpr (A8) a[t] = join(*reinterpret_cast<const v4i_t*>(base + a_lo + t * 16 * T::PA), *reinterpret_cast<const v4i_t*>(base + a_hi + t * 16 * T::PA));
-            else a[t] = widen(*reinterpret_cast<const v4i_t*>(base + a_lo + t * 16 * T::PA));
-        }
+            for (int t = 0; t < MT; ++t) {
+                if constexpr (A8) a[t] = join(*reinterpret_cast<const v4i_t*>(base + a_lo + t * 2048), *reinterpret_cast<const v4i_t*>(base + a_hi + t * 2048));
+                else a[t] = widen(*reinterpret_cast<const v4i_t*>(base + (H ? a_hi : a_lo) + t * 2048));
+            }
 #pragma unroll
-        for (int j = 0; j < NT; ++j) b[j] = widen(*reinterpret_cast<const v4i_t*>(base + b_at + frag_col<TO>(j) * 64));
+            for (int j = 0; j < NT; ++j) b[j] = widen(*reinterpret_cast<const v4i_t*>(base + (!A8 && H ? b_hi : b_lo) + frag_col<TO>(j) * T::PB));
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) mma<A8, P>(b[j], a[t], acc[t][j], bs[j], as[t]);
+                for (int t = 0; t < MT; ++t) mma<A8, H>(b[j], a[t], acc[t][j], bs[j], as[t]);
+        };
+        step(par);
+        if constexpr (!A8) step(std::integral_constant<int, 1>{});
     };
 
 #pragma unroll
     for (int k = 0; k < S - 1; ++k)
-        if (k < nk) {
-            if ((k & 1) == 0) issue_scales(k >> 1);
-            issue(k);
+        if (k < nk) issue(k);
+    constexpr std::integral_constant<int, 0> zero{};
+    constexpr std::integral_constant<int, 1> one{};
+    if constexpr (A8) {
+        for (int kt = 0; kt < nk; kt += 2) {
+            stage(zero, kt);
+            if (kt + 1 < nk) stage(one, kt + 1);
         }
-    for (int kt = 0; kt < nk; kt += 2) {
-        stage(std::integral_constant<int, 0>{}, kt);
-        if (kt + 1 < nk) stage(std::integral_constant<int, 1>{}, kt + 1);
+    } else {
+        for (int kt = 0; kt < nk; ++kt) stage(zero, kt);
     }
 
     // ---- outputs
@@ -391,22 +403,22 @@ template <bool A8, bool RS, typename TO, int WM, int WN, int MT, int NT, int S, 
     return DIST_OK;
 }
 
-enum { FEW = 0, SMALL = 1, SQUARE = 2, WIDE = 3 };
+enum { FEW = 0, SMALL = 1, SQUARE = 2, BIG = 3 };
 struct Plan { int kind, slice; };
 constexpr int LIMIT = 1 << 22;                               // bytes of a row (128 rows of a tile lie within 32-bit offsets)
 
 // Which kernel (times in us, inputs out of the caches, bias; kernels of this file beside each other):
 //   FEW     M <= 64: the tiles' ring has a long way to the first result.  N = K = 4096: 64 rows 9.1 against 10.9 in 64 x 64 tiles, 16 rows 4.8
-//   SMALL   64 x 64, where 128 x 128 would leave CUs without work (under 200 tiles): 788 x 2304 x 768 5.4 against 5.9; 2048 x 2048 x 1024 (256 tiles) 8.4 against 7.0 the other way.
+//   SMALL   64 x 64, where 128 x 128 would leave CUs without work (under 200 tiles): 788 x 2304 x 768 4.9 against 5.9; 2048 x 2048 x 1024 (256 tiles) 8.4 against 6.4 the other way.
 //           The long axis is cut where even these do not fill the 256 CUs, in slices of at least 2048 (shorter ones cost more in the joining pass than they gain:
 //           200 x 520 x 2048 7.1 whole, 7.7 in two)
-//   SQUARE  128 x 128, three workgroups a CU (768 places);  WIDE 128 x 256, two a CU (512 places), 4-bit operands only: a tile takes 1.5 times as long and does twice the work,
-//           so it is worth its places when its rounds are few enough: 4096^3 43 against 55, 6400 x 2304 x 768 13.4 against 15.6, but 16448 x 1024 x 4096 (516 tiles) 68 against 62
+//   SQUARE  128 x 128, two workgroups a CU (e4m3: three)
+//   BIG     256 x 256, one a CU, 4-bit operands only (e4m3: 30 against 28 at 12608 x 2304 x 768): four times the work of SQUARE, so it wins where its rounds over the 256 CUs are
+//           full, by 6 % and more: 4096^3 39 against 44, 6400 x 2304 x 768 (225 tiles) 12.6 against 13.4, but 16448 x 1024 x 4096 (260 tiles) 68 against 56
 Plan plan(int64_t M, int N, int K, int a_fmt) {
-    const int64_t t64 = (M + 63) / 64 * ((N + 63) / 64), t128 = (M + 127) / 128 * ((N + 127) / 128), t256 = (M + 127) / 128 * ((N + 255) / 256);
+    const int64_t t64 = (M + 63) / 64 * ((N + 63) / 64), t128 = (M + 127) / 128 * ((N + 127) / 128), t256 = (M + 255) / 256 * ((N + 255) / 256);
     if (M <= 64) return Plan{FEW, K};
-    if (t128 >= 200)
-        return Plan{a_fmt == DIST_MX_A_MXFP4 && 3 * ((t256 + 511) / 512) <= 2 * ((t128 + 767) / 768) ? WIDE : SQUARE, K};
+    if (t128 >= 200) return Plan{a_fmt == DIST_MX_A_MXFP4 && 15 * ((t256 + 255) / 256) <= 4 * ((t128 + 255) / 256) ? BIG : SQUARE, K};
     int parts = 1;
     while (t64 * parts < 256 && K / (2 * parts) >= 2048) parts *= 2;
     return Plan{SMALL, parts == 1 ? K : (K / parts + 255) / 256 * 256};
@@ -426,9 +438,10 @@ template <bool A8, typename TO> int launch(const dist_gemm_mx_args& p, hipStream
         return launch_few<A8, TO, 4, 1, 8>(p, s);
     }
     if constexpr (!A8) {
-        if (w.kind == WIDE) return launch_tile<A8, true, TO, 2, 2, 4, 8, 2, 2>(p, p.K, s);
+        constexpr bool H = sizeof(TO) == 2;                  // (32-bit outputs: 64 x 128 a wave, else the residual's eight rows do not fit in registers)
+        if (w.kind == BIG) return launch_tile<A8, true, TO, H ? 2 : 4, H ? 4 : 2, H ? 8 : 4, H ? 4 : 8, 2, 2>(p, p.K, s);
     }
-    if (w.kind == SQUARE) return launch_tile<A8, true, TO, 2, 2, 4, 4, 2, 3>(p, p.K, s);
+    if (w.kind == SQUARE) return launch_tile<A8, true, TO, 2, 2, 4, 4, 2, A8 ? 3 : 2>(p, p.K, s);
     if (w.slice >= p.K) return launch_tile<A8, true, TO, 4, 1, 1, 4, 4, 4>(p, p.K, s);
     dist_gemm_mx_args q = p;
     q.C = p.scratch;
