@@ -372,8 +372,8 @@ template <typename T, typename TD, bool AL> int bwd(const dist_rms_bwd_args& p, 
     if (!lanes) {
         if (p.rows > 0x7fffffff) return DIST_ERR_ARG;
         const int ctiles = (p.C + NT - 1) / NT;
+        hipLaunchKernelGGL((rms_dw_cols_kernel<T, TD>), dim3((unsigned)(G * ctiles)), dim3(NT), 0, s, p, G, ctiles);       // (before dh, which may take h's or dy's place)
         if (p.dh && p.rows) hipLaunchKernelGGL((rms_bwd_long_kernel<T, TD>), dim3((unsigned)p.rows), dim3(NT), 0, s, p);
-        hipLaunchKernelGGL((rms_dw_cols_kernel<T, TD>), dim3((unsigned)(G * ctiles)), dim3(NT), 0, s, p, G, ctiles);
     } else if (lanes == 16) DIST_RMS(16, 3);
     else if (lanes == 32) DIST_RMS(32, 3);
     else if (lanes == 64) { if (p.C <= 1024) DIST_RMS(64, 2); else DIST_RMS(64, 4); }

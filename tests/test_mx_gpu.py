@@ -203,6 +203,20 @@ def test_norm_gradient_many_rows_and_none(gpu_lib):
     assert ops.rmsnorm(h0, torch.ones(64, device="cuda"), fmt="e4m3")["q"].shape == (0, 64)
 
 
+@pytest.mark.parametrize("C", [300, 768, 2048, 8192, 8200, 17000])
+def test_norm_gradient_in_place_keeps_dw(C, gpu_lib):
+    # dh in the place of h or of dy: dw is of the values that were there
+    for rows in (3, 70):
+        h, d, r, w = act(rows, C, BF, 1), act(rows, C, BF, 2), act(rows, C, BF, 4), torch.rand(C, generator=gen(3)).cuda()
+        rstd = mo.rms(h, w)[1].float().cuda()
+        dh, dw = ops.rmsnorm_bwd(h, rstd, d, w, dres=r)
+        for own in (0, 1, 2):
+            c = [h.clone(), d.clone(), r.clone()]
+            got = ops.rmsnorm_bwd(c[0], rstd, c[1], w, dres=c[2], dh=c[own])
+            same_bits(got[0], dh)
+            same_bits(got[1], dw)
+
+
 # ---- quantisation ---------------------------------------------------------------------------------------------------------------------------------------------
 
 def spread(rows, K, dtype, seed):
