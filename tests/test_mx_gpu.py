@@ -360,6 +360,13 @@ def test_product_sizes_of_use(M, N, K, fmt, out, gpu_lib):
     check_product(M, N, K, fmt, out, True, True, 5)
 
 
+@pytest.mark.parametrize("M,N,K,out", [(6300, 2304, 768, BF), (6300, 2299, 288, BF), (4000, 3999, 160, F32), (3990, 4000, 544, F32), (6144, 2312, 32, BF), (6390, 2052, 1056, F32)])
+@pytest.mark.parametrize("bias,res", [(False, False), (True, True)])
+def test_product_of_large_tiles(M, N, K, out, bias, res, gpu_lib):
+    # sizes whose 256 x 256 tiles fill the chip; ragged edges, odd widths, one stage and many
+    check_product(M, N, K, "mxfp4", out, bias, res, 9)
+
+
 @pytest.mark.parametrize("M,N,K,fmt,out", [(2600, 2304, 768, "mxfp4", BF), (2600, 2304, 768, "e4m3", BF), (4096, 2304, 768, "mxfp4", F32), (2600, 2304, 1024, "mxfp4", BF), (12608, 2304, 768, "mxfp4", BF),
                                            (300, 520, 2048, "mxfp4", F32), (300, 520, 2048, "e4m3", BF)])
 @pytest.mark.parametrize("bias", [False, True])
