@@ -405,7 +405,7 @@ template <bool A8, bool RS, typename TO, int WM, int WN, int MT, int NT, int S, 
 
 enum { FEW = 0, SMALL = 1, SQUARE = 2, BIG = 3 };
 struct Plan { int kind, slice; };
-constexpr int LIMIT = 1 << 22;                               // bytes of a row (128 rows of a tile lie within 32-bit offsets)
+constexpr int LIMIT = 1 << 22;                               // bytes of a row (the 256 rows of a tile lie within 32-bit offsets)
 
 // Which kernel (times in us, inputs out of the caches, bias; kernels of this file beside each other):
 //   FEW     M <= 64: the tiles' ring has a long way to the first result.  N = K = 4096: 64 rows 9.1 against 10.9 in 64 x 64 tiles, 16 rows 4.8
@@ -413,12 +413,13 @@ constexpr int LIMIT = 1 << 22;                               // bytes of a row (
 //           The long axis is cut where even these do not fill the 256 CUs, in slices of at least 2048 (shorter ones cost more in the joining pass than they gain:
 //           200 x 520 x 2048 7.1 whole, 7.7 in two)
 //   SQUARE  128 x 128, two workgroups a CU (e4m3: three)
-//   BIG     256 x 256, one a CU, 4-bit operands only (e4m3: 30 against 28 at 12608 x 2304 x 768): four times the work of SQUARE, so it wins where its rounds over the 256 CUs are
-//           full, by 6 % and more: 4096^3 39 against 44, 6400 x 2304 x 768 (225 tiles) 12.6 against 13.4, but 16448 x 1024 x 4096 (260 tiles) 68 against 56
-Plan plan(int64_t M, int N, int K, int a_fmt) {
+//   BIG     256 x 256, one a CU: four times the work of SQUARE, so it wins where its rounds over the 256 CUs are full, by 6 % and more.  4-bit rows: 4096^3 39 against 44,
+//           6400 x 2304 x 768 (225 tiles) 12.6 against 13.4, but 16448 x 1024 x 4096 (260 tiles) 68 against 56;  e4m3 rows: 8192^3 380 (2.9 PF) against 414,
+//           50432 x 2304 x 768 101 against 104, 16384 x 1024 x 4096 56 against 63, but 12608 x 2304 x 768 (450 tiles) 29 against 27
+Plan plan(int64_t M, int N, int K) {
     const int64_t t64 = (M + 63) / 64 * ((N + 63) / 64), t128 = (M + 127) / 128 * ((N + 127) / 128), t256 = (M + 255) / 256 * ((N + 255) / 256);
     if (M <= 64) return Plan{FEW, K};
-    if (t128 >= 200) return Plan{a_fmt == DIST_MX_A_MXFP4 && 15 * ((t256 + 255) / 256) <= 4 * ((t128 + 255) / 256) ? BIG : SQUARE, K};
+    if (t128 >= 200) return Plan{15 * ((t256 + 255) / 256) <= 4 * ((t128 + 255) / 256) ? BIG : SQUARE, K};
     int parts = 1;
     while (t64 * parts < 256 && K / (2 * parts) >= 2048) parts *= 2;
     return Plan{SMALL, parts == 1 ? K : (K / parts + 255) / 256 * 256};
@@ -431,16 +432,15 @@ template <bool A8, typename TO, int MT, int NT, int W> int launch_few(const dist
 }
 
 template <bool A8, typename TO> int launch(const dist_gemm_mx_args& p, hipStream_t s) {
-    Plan w = plan(p.M, p.N, p.K, p.a_fmt);
+    Plan w = plan(p.M, p.N, p.K);
     if (w.kind == FEW) {
         if (p.M <= 16) return launch_few<A8, TO, 1, 1, 8>(p, s);
         if (p.M <= 32) return launch_few<A8, TO, 2, 1, 8>(p, s);
         return launch_few<A8, TO, 4, 1, 8>(p, s);
     }
-    if constexpr (!A8) {
-        constexpr bool H = sizeof(TO) == 2;                  // (32-bit outputs: 64 x 128 a wave, else the residual's eight rows do not fit in registers)
-        if (w.kind == BIG) return launch_tile<A8, true, TO, H ? 2 : 4, H ? 4 : 2, H ? 8 : 4, H ? 4 : 8, 2, 2>(p, p.K, s);
-    }
+    // (64 x 128 a wave where 128 x 64 needs more registers: e4m3 fragments, fp32 residuals)
+    constexpr bool TALL = !A8 && sizeof(TO) == 2;
+    if (w.kind == BIG) return launch_tile<A8, true, TO, TALL ? 2 : 4, TALL ? 4 : 2, TALL ? 8 : 4, TALL ? 4 : 8, 2, 2>(p, p.K, s);
     if (w.kind == SQUARE) return launch_tile<A8, true, TO, 2, 2, 4, 4, 2, A8 ? 3 : 2>(p, p.K, s);
     if (w.slice >= p.K) return launch_tile<A8, true, TO, 4, 1, 1, 4, 4, 4>(p, p.K, s);
     dist_gemm_mx_args q = p;
@@ -459,7 +459,7 @@ template <bool A8, typename TO> int launch(const dist_gemm_mx_args& p, hipStream
 
 extern "C" int64_t dist_op_gemm_mxfp4_scratch(int64_t M, int N, int K, int a_fmt) {
     if (M < 0 || N <= 0 || K <= 0 || K % 32 || (a_fmt != DIST_MX_A_MXFP4 && a_fmt != DIST_MX_A_E4M3)) return -1;
-    const Plan w = plan(M, N, K, a_fmt);
+    const Plan w = plan(M, N, K);
     const int64_t parts = (K + w.slice - 1) / w.slice;
     return parts > 1 ? parts * M * N : 0;
 }

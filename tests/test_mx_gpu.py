@@ -365,6 +365,8 @@ def test_product_sizes_of_use(M, N, K, fmt, out, gpu_lib):
 def test_product_of_large_tiles(M, N, K, out, bias, res, gpu_lib):
     # sizes whose 256 x 256 tiles fill the chip; ragged edges, odd widths, one stage and many
     check_product(M, N, K, "mxfp4", out, bias, res, 9)
+    if out == BF:
+        check_product(M, N, K, "e4m3", out, bias, res, 9)
 
 
 @pytest.mark.parametrize("M,N,K,fmt,out", [(2600, 2304, 768, "mxfp4", BF), (2600, 2304, 768, "e4m3", BF), (4096, 2304, 768, "mxfp4", F32), (2600, 2304, 1024, "mxfp4", BF), (12608, 2304, 768, "mxfp4", BF),
