@@ -102,10 +102,10 @@ __global__ __launch_bounds__(64 * W) void gemm_mx_few_kernel(const dist_gemm_mx_
 // them first.  A 16-byte chunk c of row r lies at chunk c ^ f(r), applied where the DMA reads (its LDS side is lane-linear).  Descriptors end behind the last row, and chunks
 // behind K are sent past the end: all of these read as zeros.
 // Measured (50432 x 2304 x 768, 4-bit operands, bf16 out): 83 us = 2.15 PF (stages of 128 elements: 95); of it 43 us are the outputs' stores (5.4 TB/s), which with three
-// stages a tile add to the loop more than they hide behind it.  4096^3: 39 us = 3.5 PF.  Deep (16448 x 1024 x 4096, e4m3): 78 us = 1.8 PF, by the 41 GB/s a CU draws through
-// its LDS-DMA.
-// Built and not faster (in stages of 128): workgroups that stay and prefetch across tiles, fragments read half a stage ahead, three or four stages in the ring, all reads in
-// front of the matrix instructions, raised priority around them (all within 5 %).
+// stages a tile add to the loop more than they hide behind it.  4096^3: 38 us = 3.6 PF.  e4m3 rows: 8192^3 379 us = 2.9 PF; 24576 x 1024 x 4096 98 us = 2.1 PF, the matrix
+// units busy 54 % of the clocks (1.87 GHz) and the LDS reads 23 %: the three workgroups of a CU wait at their barriers at much the same time.
+// Built and not faster: workgroups that stay and prefetch across tiles (in both depths of stages); in stages of 128 fragments read half a stage ahead, three or four stages in
+// the ring, all reads in front of the matrix instructions, raised priority around them (all within 5 %).
 typedef __attribute__((address_space(3))) void* lds_ptr;
 DEV void regs_pin(unsigned& v) { asm volatile("" : "+v"(v)); }
 template <int N> DEV void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
