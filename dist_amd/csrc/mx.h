@@ -52,32 +52,68 @@ DEV void unpack8(unsigned w, int byte, float v[8]) {
 // of 1411 fp32 take the norm 9.7 us so, 12.6 by single elements).
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
 template <typename T> struct __attribute__((packed)) Loose { T v[8]; };
-template <bool AL, typename T> struct Raw8 {                   // as they were read, for loads that run ahead
+template <bool AL, typename T> DEV void load8(const T* p, long n, float o[8]) {
     Frag<T> f;
-    DEV void load(const T* p, long n) {
-        if (n >= 8) {
-            if constexpr (AL) frag_load(f, p);
-            else {
-                const Loose<T> u = *reinterpret_cast<const Loose<T>*>(p);
-                f = __builtin_bit_cast(Frag<T>, u);
-            }
-        } else {
-            frag_zero(f);
-            if constexpr (!AL) {
+    if (n >= 8) {
+        if constexpr (AL) frag_load(f, p);
+        else {
+            const Loose<T> u = *reinterpret_cast<const Loose<T>*>(p);
+            f = __builtin_bit_cast(Frag<T>, u);
+        }
+    } else {
+        frag_zero(f);
+        if constexpr (!AL) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (e < n) frag_set(f, e, to_f(p[e]));
+            for (int e = 0; e < 8; ++e)
+                if (e < n) frag_set(f, e, to_f(p[e]));
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = frag_get(f, e);
+}
+// The same for loads that run ahead, from rows of eight elements at least: a partial group is read as the row's last eight elements, and settle() moves them into place
+// when they are used.  (Zeros or single elements written into a load's registers under another mask wait for that load: 10630 rows of 1411 bf16 took the norm's gradient
+// 64 us so, and take it 38.)
+template <bool AL, typename T> struct Raw8 {
+    Frag<T> f;
+    DEV Raw8() { frag_zero(f); }
+    DEV void load(const T* p, long n) {
+        if (n <= 0) return;
+        if constexpr (AL) frag_load(f, p);
+        else {
+            const Loose<T> u = *reinterpret_cast<const Loose<T>*>(n < 8 ? p + (n - 8) : p);
+            f = __builtin_bit_cast(Frag<T>, u);
+        }
+    }
+    DEV void settle(long n) {
+        if constexpr (!AL) {
+            constexpr int W = sizeof(T) == 2 ? 4 : 8, E = 8 / W;        // words, elements of a word
+            struct Words { unsigned w[W]; };
+            Words q = __builtin_bit_cast(Words, f);
+#pragma unroll
+            for (int i = 0; i < W; ++i) asm volatile("" : "+v"(q.w[i]));       // (not in front of the loads' arrival: hipcc moves it up to them)
+            if (n < 8) {
+                const int k = n > 0 ? 8 - (int)n : 8;                // down by k elements, zeros behind them
+#pragma unroll
+                for (int bit = 4; bit >= E; bit >>= 1)
+#pragma unroll
+                    for (int i = 0; i < W; ++i) {
+                        const unsigned up = i + bit / E < W ? q.w[i + bit / E] : 0u;
+                        q.w[i] = k == 8 ? 0u : k & bit ? up : q.w[i];
+                    }
+                if constexpr (E == 2) {
+#pragma unroll
+                    for (int i = 0; i < W; ++i) {
+                        const unsigned up = i + 1 < W ? q.w[i + 1] : 0u;
+                        q.w[i] = k & 1 ? q.w[i] >> 16 | up << 16 : q.w[i];
+                    }
+                }
             }
+            f = __builtin_bit_cast(Frag<T>, q);
         }
     }
     DEV float get(int e) const { return frag_get(f, e); }
 };
-template <bool AL, typename T> DEV void load8(const T* p, long n, float o[8]) {
-    Raw8<AL, T> r;
-    r.load(p, n);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = r.get(e);
-}
 // stores: past the caches' keeping where rows are aligned (outputs that a later kernel reads from memory anyway)
 template <bool AL, typename T> DEV void store8(T* p, long n, const float o[8]) {
     Frag<T> f;

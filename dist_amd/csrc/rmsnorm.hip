@@ -10,14 +10,16 @@ namespace {
 
 constexpr int NT = 256;
 
-// sum / maximum over the LPR lanes that own a row; every lane gets the result.  LPR = 256: the whole block, `red` = 4 words of LDS, fixed order
+// sum / maximum over the LPR lanes that own a row; every lane gets the result.  LPR = 256 or 512: the whole block, `red` = 4 or 8 words of LDS, fixed order
 template <int LPR> DEV float row_sum(float v, float* red) {
     if constexpr (LPR <= 64) return wave_sum(v, LPR);
     v = wave_sum(v, 64);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
+    const float s = (red[0] + red[1]) + (red[2] + red[3]);
+    if constexpr (LPR == 512) return s + ((red[4] + red[5]) + (red[6] + red[7]));
+    return s;
 }
 template <int LPR> DEV float row_max(float v, float* red) {
     if constexpr (LPR <= 64) return wave_max(v, LPR);
@@ -188,11 +190,11 @@ __global__ __launch_bounds__(NT) void rms_fwd_long_kernel(const dist_rms_args p)
 // Backward.  A block keeps the sums of dw over its rows in registers and leaves one partial row; rms_dw_kernel adds the partial rows in a fixed order (no atomics:
 // the same bits every time).
 template <typename T, typename TD, bool AL, int LPR, int IT>
-__global__ __launch_bounds__(NT) void rms_bwd_kernel(const dist_rms_bwd_args p) {
-    __shared__ float red[4];
+__global__ __launch_bounds__(LPR > NT ? LPR : NT, 2) void rms_bwd_kernel(const dist_rms_bwd_args p) {
+    __shared__ float red[8];
     __shared__ float cols[LPR < NT ? LPR * IT * 8 : 1];
     const int lr = threadIdx.x % LPR, slot = threadIdx.x / LPR, C = p.C;
-    constexpr int RPB = NT / LPR;
+    constexpr int RPB = LPR < NT ? NT / LPR : 1;
     float w[IT][8], aw[IT][8];
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
@@ -224,13 +226,18 @@ __global__ __launch_bounds__(NT) void rms_bwd_kernel(const dist_rms_bwd_args p) 
         const float rstd = sn;
         float n[IT][8], g[IT][8], o[IT][8];
 #pragma unroll
-        for (int it = 0; it < IT; ++it)
+        for (int it = 0; it < IT; ++it) {
+            const int c = (lr + it * LPR) * 8;
+            hn[it].settle(C - c);
+            dn[it].settle(C - c);
+            if (A) rn[it].settle(C - c);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 n[it][e] = hn[it].get(e) * rstd;
                 g[it][e] = dn[it].get(e);
                 o[it][e] = A ? rn[it].get(e) : 0.f;
             }
+        }
         if (row + stride < p.rows) fetch(row + stride);
         float s = 0.f;
 #pragma unroll
@@ -256,7 +263,7 @@ __global__ __launch_bounds__(NT) void rms_bwd_kernel(const dist_rms_bwd_args p) 
     // the only workgroup (few rows) writes dw itself
     const bool only = gridDim.x == 1, add = only && p.accumulate;
     float* part = only ? p.dw : p.scratch + (long)blockIdx.x * C;
-    if constexpr (LPR == NT) {
+    if constexpr (LPR >= NT) {
 #pragma unroll
         for (int it = 0; it < IT; ++it) {
             const int c = (lr + it * LPR) * 8;
@@ -329,11 +336,12 @@ __global__ __launch_bounds__(1024) void rms_dw_kernel(const float* __restrict__ 
 constexpr int FWD_MAX = 16384, BWD_MAX = 8192;                // widths whose rows stay in registers
 constexpr int PARTIALS = 512;                                  // workgroups of the backward kernel, two a CU (50432 x 768: 384 67 us, 512 62, 640 77, 1024 66)
 
-// lanes per row of the backward kernel (0: a long row)
-inline int bwd_lanes(int C) { return C <= 384 ? 16 : C <= 768 ? 32 : C <= 2048 ? 64 : C <= BWD_MAX ? 256 : 0; }
+// lanes per row of the backward kernel (0: a long row, or one of less than a group).  At most three groups of eight a lane, else a CU holds one workgroup only (15 M elements in bf16: 2048 columns by 64 lanes
+// of four groups 29.6 us, by 256 of one 27.6; 8192 by 256 of four 40.3, by 512 of two 38.6)
+inline int bwd_lanes(int C) { return C < 8 ? 0 : C <= 384 ? 16 : C <= 768 ? 32 : C <= 1024 ? 64 : C <= 4096 ? 256 : C <= BWD_MAX ? 512 : 0; }
 inline int64_t bwd_partials(int64_t rows, int C) {
     const int lanes = bwd_lanes(C);
-    const int64_t per = lanes ? NT / lanes : 1, need = (rows + per - 1) / per, most = lanes ? PARTIALS : 64;
+    const int64_t per = lanes && lanes < NT ? NT / lanes : 1, need = (rows + per - 1) / per, most = lanes ? PARTIALS : 64;
     if (lanes && need <= 4) return 1;                         // (few rows: a second launch costs more than a workgroup's four steps)
     return need < 1 ? 1 : need > most ? most : need;
 }
@@ -368,7 +376,7 @@ template <typename T, int FMT> int fwd(const dist_rms_args& p, hipStream_t s) {
 template <typename T, typename TD, bool AL> int bwd(const dist_rms_bwd_args& p, hipStream_t s) {
     const int G = (int)bwd_partials(p.rows, p.C);
     const int lanes = bwd_lanes(p.C);
-#define DIST_RMS(LPR, IT) hipLaunchKernelGGL((rms_bwd_kernel<T, TD, AL, LPR, IT>), dim3((unsigned)G), dim3(NT), 0, s, p)
+#define DIST_RMS(LPR, IT) hipLaunchKernelGGL((rms_bwd_kernel<T, TD, AL, LPR, IT>), dim3((unsigned)G), dim3(LPR > NT ? LPR : NT), 0, s, p)
     if (!lanes) {
         if (p.rows > 0x7fffffff) return DIST_ERR_ARG;
         const int ctiles = (p.C + NT - 1) / NT;
@@ -376,8 +384,9 @@ template <typename T, typename TD, bool AL> int bwd(const dist_rms_bwd_args& p, 
         if (p.dh && p.rows) hipLaunchKernelGGL((rms_bwd_long_kernel<T, TD>), dim3((unsigned)p.rows), dim3(NT), 0, s, p);
     } else if (lanes == 16) DIST_RMS(16, 3);
     else if (lanes == 32) DIST_RMS(32, 3);
-    else if (lanes == 64) { if (p.C <= 1024) DIST_RMS(64, 2); else DIST_RMS(64, 4); }
-    else { if (p.C <= 4096) DIST_RMS(256, 2); else DIST_RMS(256, 4); }
+    else if (lanes == 64) DIST_RMS(64, 2);
+    else if (lanes == 256) { if (p.C <= 2048) DIST_RMS(256, 1); else DIST_RMS(256, 2); }
+    else DIST_RMS(512, 2);
 #undef DIST_RMS
     HIP_CHECK_RET(hipGetLastError());
     if (lanes && G == 1) return DIST_OK;

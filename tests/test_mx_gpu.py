@@ -173,6 +173,13 @@ def test_norm_gradient(C, dtype, dyt, gpu_lib):
         same_bits(ops.rmsnorm_bwd(c[0], rstd, c[1], w, dres=c[2], dh=out)[0], dh)
 
 
+@pytest.mark.parametrize("dtype,dyt", [(BF, BF), (F32, F32)])
+@pytest.mark.parametrize("C", [2, 5, 7, 9, 10, 11, 12, 13, 14, 15, 390, 1025, 1031, 2049, 4095, 5001, 8191])
+def test_norm_gradient_of_partial_groups(C, dtype, dyt, gpu_lib):
+    # every length of a row's last group, and rows shorter than one
+    test_norm_gradient(C, dtype, dyt, gpu_lib)
+
+
 def test_norm_gradient_many_rows_and_none(gpu_lib):
     for rows, C, dt in ((9001, 768, BF), (4999, 100, F32), (70, 9000, BF)):
         h, d, w = act(rows, C, dt, 1), act(rows, C, dt, 2), torch.rand(C, generator=gen(3)).cuda()
