@@ -214,7 +214,7 @@ DEV void fast_epilogue(const dist_gemm_args& p, f32x4 (&acc)[8][4], char* smem, 
     // STORED behind the next block's (the LDS round trip hides behind that block's arithmetic instead of stalling every piece)
     __amdgpu_buffer_rsrc_t rd1 = __builtin_amdgcn_make_buffer_rsrc(dst1, 0, 0, 0x00020000);
     unsigned off1 = 0, fs_adj = 0;
-    int step1 = 0;
+    unsigned step1 = 0;
     if constexpr (SPEC) {
         if (heads_om) {
             const unsigned fs = (unsigned)p.omap.p1 * 3u * (unsigned)p.omap.p0 * 128u;      // bytes per frame: [head][q|k|v][token][64]
@@ -224,21 +224,22 @@ DEV void fast_epilogue(const dist_gemm_args& p, f32x4 (&acc)[8][4], char* smem, 
         } else {
             rd1 = __builtin_amdgcn_make_buffer_rsrc(dst1, 0, nw < N ? M * ld1 * 2 : 0, 0x00020000);
             off1 = (unsigned)(mw + crow) * (unsigned)ld1 * 2u + (unsigned)(nw + cchunk * 8) * 2u;
-            step1 = 8 * ld1 * 2;
+            step1 = 8u * (unsigned)ld1 * 2u;
         }
     }
     auto ld_piece = [&](const int it) __attribute__((always_inline)) {
         const int r = it * 8 + crow;
         return *reinterpret_cast<const v4u_t*>(erow(r) + ((cchunk ^ (r & 7)) << 4));
     };
-    auto st_piece = [&](const int it, const v4u_t& v) __attribute__((always_inline)) {      // (pieces in order 0 ... 15: the head-major offset is stepped)
+    // pieces in order 0 ... 15: the lanes' offset is stepped.  (Never the scalar offset: behind a 16-byte store whose scalar offset is a register hipcc may write the
+    // store's data anew in the very next instruction, and gfx950 then stores the new value in some lanes.)
+    auto st_piece = [&](const v4u_t& v) __attribute__((always_inline)) {
+        if (DIST_AB && (dbg & 4)) __builtin_amdgcn_raw_buffer_store_b128(v, rd1, off1, 0, 0);      // (timing-only library: without the streaming hint)
+        else __builtin_amdgcn_raw_buffer_store_b128(v, rd1, off1, 0, 2);
         if (heads_om) {
-            if (DIST_AB && (dbg & 4)) __builtin_amdgcn_raw_buffer_store_b128(v, rd1, off1, 0, 0);      // (timing-only library: without the streaming hint)
-            else __builtin_amdgcn_raw_buffer_store_b128(v, rd1, off1, 0, 2);
             htok1 += 8; off1 += 1024u;
             if (htok1 >= p.omap.p0) { htok1 -= p.omap.p0; off1 += fs_adj; }                 // (the launcher checks p0 >= 16)
-        } else if (DIST_AB && (dbg & 4)) __builtin_amdgcn_raw_buffer_store_b128(v, rd1, off1, it * step1, 0);
-        else __builtin_amdgcn_raw_buffer_store_b128(v, rd1, off1, it * step1, 2);
+        } else off1 += step1;
     };
     v4u_t pend0 = {0, 0, 0, 0}, pend1 = {0, 0, 0, 0};
     // the residual values of row block i + 1 are read from the staging region BEFORE block i's results are written to it (the compiler keeps LDS
@@ -289,19 +290,19 @@ DEV void fast_epilogue(const dist_gemm_args& p, f32x4 (&acc)[8][4], char* smem, 
         }
         if constexpr (SPEC) {
             if (dst1 && early) {
-                if (i > 0) { st_piece(2 * i - 2, pend0); st_piece(2 * i - 1, pend1); }
+                if (i > 0) { st_piece(pend0); st_piece(pend1); }
                 pend0 = ld_piece(2 * i); pend1 = ld_piece(2 * i + 1);
             }
         } else if (dst1 && early) { flush_piece(2 * i); flush_piece(2 * i + 1); }
     }
     if constexpr (SPEC) {
-        if (dst1 && early) { st_piece(14, pend0); st_piece(15, pend1); }
+        if (dst1 && early) { st_piece(pend0); st_piece(pend1); }
         else if (dst1) {                                  // all 16 pieces behind the last conversion: 16 reads, then 16 stores
             v4u_t pv[16];
 #pragma unroll
             for (int it = 0; it < 16; ++it) pv[it] = ld_piece(it);
 #pragma unroll
-            for (int it = 0; it < 16; ++it) st_piece(it, pv[it]);
+            for (int it = 0; it < 16; ++it) st_piece(pv[it]);
         }
     } else if (dst1 && !early) {                          // all 16 pieces behind the last conversion
 #pragma unroll
@@ -360,8 +361,7 @@ DEV void fast_epilogue(const dist_gemm_args& p, f32x4 (&acc)[8][4], char* smem, 
         if constexpr (SPEC) {                             // (compile-time epilogue: the image's rows through a buffer descriptor, as the primary output's)
             const int pc = lane & 3;
             __amdgpu_buffer_rsrc_t r8;
-            unsigned off8, adj8 = 0;
-            int step8 = 0;
+            unsigned off8, adj8 = 0, step8 = 0;
             if (heads_om) {
                 const unsigned fs = (unsigned)p.omap.p1 * 3u * (unsigned)p.omap.p0 * 64u;   // bytes per frame
                 r8 = __builtin_amdgcn_make_buffer_rsrc(C8, 0, nw < N ? (int)((unsigned)(M / p.omap.p0) * fs) : 0, 0x00020000);
@@ -370,7 +370,7 @@ DEV void fast_epilogue(const dist_gemm_args& p, f32x4 (&acc)[8][4], char* smem, 
             } else {
                 r8 = __builtin_amdgcn_make_buffer_rsrc(C8, 0, nw < N ? M * p.ldc8 : 0, 0x00020000);
                 off8 = (unsigned)(mw + (lane >> 2)) * (unsigned)p.ldc8 + (unsigned)(nw + pc * 16);
-                step8 = 16 * p.ldc8;
+                step8 = 16u * (unsigned)p.ldc8;
             }
             v4u_t pv8[8];
 #pragma unroll
@@ -380,11 +380,11 @@ DEV void fast_epilogue(const dist_gemm_args& p, f32x4 (&acc)[8][4], char* smem, 
             }
 #pragma unroll
             for (int it = 0; it < 8; ++it) {
+                __builtin_amdgcn_raw_buffer_store_b128(pv8[it], r8, off8, 0, 2);
                 if (heads_om) {
-                    __builtin_amdgcn_raw_buffer_store_b128(pv8[it], r8, off8, 0, 2);
                     htok += 16; off8 += 1024u;
                     if (htok >= p.omap.p0) { htok -= p.omap.p0; off8 += adj8; }
-                } else __builtin_amdgcn_raw_buffer_store_b128(pv8[it], r8, off8, it * step8, 2);
+                } else off8 += step8;
             }
         } else
 #pragma unroll
