@@ -600,11 +600,28 @@ def _vector(t, n, what):
         _refuse(f"{what}: expected {n} contiguous float32 values, got {t.dtype} {tuple(t.shape)}")
 
 
+def _runs(t):
+    """(address, bytes of a run, bytes from run to run, runs) of a tensor that is contiguous, or a matrix of contiguous rows"""
+    es = t.element_size()
+    if t.dim() == 2 and t.shape[0] > 1 and t.stride(0) != t.shape[1]:
+        return t.data_ptr(), t.shape[1] * es, t.stride(0) * es, t.shape[0]
+    return t.data_ptr(), t.numel() * es, 0, 1
+
+
+def _meet(a, b):
+    """whether two tensors share a byte.  Exact for rows of one pitch (columns of one buffer lie beside each other); of different pitches: whether their spans meet"""
+    a0, aw, ap, an = _runs(a)
+    b0, bw, bp, bn = _runs(b)
+    if b0 >= a0 + (an - 1) * ap + aw or a0 >= b0 + (bn - 1) * bp + bw:
+        return False
+    if ap == bp == 0 or (ap and bp and ap != bp):
+        return True
+    at = (b0 - a0) % (ap or bp)                 # where b's runs begin between a's
+    return at < aw or at + bw > (ap or bp)
+
+
 def _apart(out, what, *inputs, may_be=True):
     """an output that the caller brings may be one of the inputs itself (same address, type, shape and pitch) but must not overlap them otherwise"""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
-
     if out.numel() == 0:
         return
     for t in inputs:
@@ -612,8 +629,7 @@ def _apart(out, what, *inputs, may_be=True):
             continue
         if may_be and out.data_ptr() == t.data_ptr() and out.dtype == t.dtype and out.shape == t.shape and (out.shape[0] == 1 or out.stride(0) == t.stride(0)):
             continue
-        a, b = span(out), span(t)
-        if a[0] < b[1] and b[0] < a[1]:
+        if _meet(out, t):
             _refuse(f"{what} overlaps an input without being it")
 
 
