@@ -602,16 +602,16 @@ def _vector(t, n, what):
 
 def _runs(t):
     """(address, bytes of a run, bytes from run to run, runs) of a tensor that is contiguous, or a matrix of contiguous rows"""
+    if t.is_contiguous():
+        return t.data_ptr(), t.nbytes, 0, 1
     es = t.element_size()
-    if t.dim() == 2 and t.shape[0] > 1 and t.stride(0) != t.shape[1]:
-        return t.data_ptr(), t.shape[1] * es, t.stride(0) * es, t.shape[0]
-    return t.data_ptr(), t.numel() * es, 0, 1
+    return t.data_ptr(), t.shape[1] * es, t.stride(0) * es, t.shape[0]
 
 
 def _meet(a, b):
-    """whether two tensors share a byte.  Exact for rows of one pitch (columns of one buffer lie beside each other); of different pitches: whether their spans meet"""
-    a0, aw, ap, an = _runs(a)
-    b0, bw, bp, bn = _runs(b)
+    """whether two tensors' runs (not empty) share a byte.  Exact for rows of one pitch (columns of one buffer lie beside each other); of different pitches: whether their spans meet"""
+    a0, aw, ap, an = a
+    b0, bw, bp, bn = b
     if b0 >= a0 + (an - 1) * ap + aw or a0 >= b0 + (bn - 1) * bp + bw:
         return False
     if ap == bp == 0 or (ap and bp and ap != bp):
@@ -621,16 +621,17 @@ def _meet(a, b):
 
 
 def _apart(out, what, *inputs, may_be=True):
-    """an output that the caller brings may be one of the inputs itself (same address, type, shape and pitch) but must not overlap them otherwise"""
-    if out.numel() == 0:
-        return
+    """an output that the caller brings may be one of these operands itself (same address, type, shape and pitch; not with may_be=False) but must not overlap them otherwise"""
+    mine = _runs(out)
+    end = mine[0] + (mine[3] - 1) * mine[2] + mine[1]
     for t in inputs:
-        if t is None or t.numel() == 0:
+        if t is None or t.data_ptr() >= end:
             continue
-        if may_be and out.data_ptr() == t.data_ptr() and out.dtype == t.dtype and out.shape == t.shape and (out.shape[0] == 1 or out.stride(0) == t.stride(0)):
+        if may_be and mine[0] == t.data_ptr() and out.dtype == t.dtype and out.shape == t.shape and (out.shape[0] == 1 or out.stride(0) == t.stride(0)):
             continue
-        if _meet(out, t):
-            _refuse(f"{what} overlaps an input without being it")
+        other = _runs(t)
+        if mine[1] and other[1] and _meet(mine, other):
+            _refuse(f"{what} overlaps another operand" + (" without being it" if may_be else ""))
 
 
 def _new(like, dense, dtype):
@@ -675,12 +676,15 @@ def rmsnorm(x, w, *, res=None, fmt="same", h=None, rstd=None, eps=1e-6):
     if rstd is not None:
         _vector(rstd, rows, "rstd")
     ldres = _matrix(res, shape, "res", dtype) if res is not None else 0
-    dev = _device(x, w, res, h, rstd)
-    out, dense = {}, x.is_contiguous()
     if h is not None:
         ldh = _matrix(h, shape, "h", dtype)
         _apart(h, "h", x, res)
-    elif res is not None:
+        _apart(h, "h", w, may_be=False)
+    if rstd is not None:
+        _apart(rstd, "rstd", x, res, w, h, may_be=False)
+    dev = _device(x, w, res, h, rstd)
+    out, dense = {}, x.is_contiguous()
+    if h is None and res is not None:
         h, ldh = _new(x, dense, dtype), Cc
     if h is not None:
         out["h"] = h
@@ -711,17 +715,19 @@ def rmsnorm_bwd(h, rstd, dy, w, *, dres=None, dh=None, dw=None):
     _vector(w, Cc, "w")
     _vector(rstd, rows, "rstd")
     lddres = _matrix(dres, shape, "dres", dtype) if dres is not None else 0
+    if dh is not None:
+        lddh = _matrix(dh, shape, "dh", dtype)
+        _apart(dh, "dh", h, dy, dres)
+        _apart(dh, "dh", rstd, w, may_be=False)
+    if dw is not None:
+        _vector(dw, Cc, "dw")
+        _apart(dw, "dw", h, rstd, dy, w, dres, dh, may_be=False)
     dev = _device(h, rstd, dy, w, dres, dh, dw)
     if dh is None:
         dh, lddh = _new(h, h.is_contiguous(), dtype), Cc
-    else:
-        lddh = _matrix(dh, shape, "dh", dtype)
-        _apart(dh, "dh", h, dy, dres)
     accumulate = int(dw is not None)
     if dw is None:
         dw = torch.empty(Cc, dtype=torch.float32, device=h.device)
-    else:
-        _vector(dw, Cc, "dw")
     lib = L.load()
     n = lib.dist_op_rmsnorm_bwd_scratch(rows, Cc)
     scratch = torch.empty(n, dtype=torch.float32, device=h.device)
@@ -782,19 +788,19 @@ def gemm_mxfp4(A, B, *, bias=None, res=None, out=None, out_dtype=torch.bfloat16)
         if Ka != K:
             _refuse(f"A has {Ka} elements a row, B has {K}")
         fmt, lda = L.MX_A_MXFP4, 0
+    if bias is not None:
+        _vector(bias, N, "bias")
+    ldres = _matrix(res, (M, N), "res", out_dtype if out is None else out.dtype) if res is not None else 0
+    if out is not None:
+        ldc = _matrix(out, (M, N), "out", out.dtype)
+        _apart(out, "out", res)
+        _apart(out, "out", q, sc, *B, bias, may_be=False)
     dev = _device(q, sc, B[0], B[1], bias, res, out)
     if out is None:
         out, ldc = torch.empty(M, N, dtype=out_dtype, device=q.device), N
-    else:
-        ldc = _matrix(out, (M, N), "out", out.dtype)
-        _apart(out, "out", res)
-        _apart(out, "out", q, B[0], may_be=False)
     dt = _dt(out)
     if fmt == L.MX_A_E4M3 and dt != L.BF16:
         _refuse("a product with an e4m3 operand gives bf16")
-    if bias is not None:
-        _vector(bias, N, "bias")
-    ldres = _matrix(res, (M, N), "res", out.dtype) if res is not None else 0
     lib = L.load()
     n = lib.dist_op_gemm_mxfp4_scratch(M, N, K, fmt) if M > 64 else 0
     scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None

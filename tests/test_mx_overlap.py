@@ -50,10 +50,56 @@ def test_meeting_is_exact_for_one_pitch_and_never_missed():
         pa = n(1, 40)
         pb = pa if n(0, 3) else n(1, 40)
         a, b = view(pa), view(pb)
-        real, said = bool(_bytes(a) & _bytes(b)), ops._meet(a, b)
+        real, said = bool(_bytes(a) & _bytes(b)), ops._meet(ops._runs(a), ops._runs(b))
         assert said or not real
         runs = ops._runs(a)[2], ops._runs(b)[2]
         if 0 in runs or runs[0] == runs[1]:
             assert said == real
             both[real] += 1
     assert min(both) > 500
+
+
+def _share(shape, dtype, other, at=0):
+    """a tensor of this shape and type in `other`'s memory, `at` bytes behind its start"""
+    n = torch.empty(shape, dtype=dtype).numel() * dtype.itemsize
+    return other.view(-1).view(torch.uint8)[at:at + n].view(dtype).view(shape)
+
+
+def test_every_buffer_is_checked_against_every_operand():
+    """(CPU tensors: the refusal comes before the one of their place, which a call without an overlap ends with)"""
+    F = torch.float32
+    C, rows, N = 64, 16, 64
+    x, r, w, rs = torch.zeros(rows, C), torch.zeros(rows, C), torch.zeros(C), torch.zeros(rows)
+    d, dw, dh = torch.zeros(rows, C), torch.zeros(C), torch.zeros(rows, C)
+    q, sa = torch.zeros(N, 32, dtype=torch.uint8), torch.zeros(1, N, 8, dtype=torch.uint8)
+    B, sb = torch.zeros(N, 32, dtype=torch.uint8), torch.zeros(1, N, 8, dtype=torch.uint8)
+    q8, s8 = torch.zeros(4, C, dtype=torch.uint8), torch.zeros(256)[:4]
+    big = torch.zeros(4096)                                          # (longer than any operand, which lie in it)
+    bf = torch.bfloat16
+    h = torch.zeros(rows, C)
+
+    def wide(t):
+        """the operand moved into `big`, behind the place of the output"""
+        return _share(t.shape, t.dtype, big)
+
+    calls = [
+        lambda: ops.rmsnorm(x, w, rstd=_share((rows,), F, x)), lambda: ops.rmsnorm(x, w, res=r, rstd=_share((rows,), F, r, 128)), lambda: ops.rmsnorm(x, w, rstd=w[:rows]),
+        lambda: ops.rmsnorm(x, w, h=h, rstd=_share((rows,), F, h, 64)), lambda: ops.rmsnorm(x, wide(w), h=_share((rows, C), F, big)), lambda: ops.rmsnorm(x, w, h=h[:], res=_share((rows, C), F, big), rstd=_share((rows,), F, big)),
+        lambda: ops.rmsnorm_bwd(h, rs, d, wide(w), dh=_share((rows, C), F, big)), lambda: ops.rmsnorm_bwd(h, wide(rs), d, w, dh=_share((rows, C), F, big)),
+        lambda: ops.rmsnorm_bwd(h, rs, d, w, dh=dh, dw=_share((C,), F, dh)), lambda: ops.rmsnorm_bwd(h, rs, d, w, dw=w), lambda: ops.rmsnorm_bwd(h, rs, d, w, dw=_share((C,), F, h, 256)),
+        lambda: ops.rmsnorm_bwd(h, rs, d, w, dw=_share((C,), F, d)), lambda: ops.rmsnorm_bwd(h, rs, d, w, dres=r, dw=_share((C,), F, r)),
+        lambda: ops.rmsnorm_bwd(h[:, :16], _share((rows,), F, big), d[:, :16], w[:16], dw=_share((16,), F, big)),
+        lambda: ops.gemm_mxfp4((q, sa), (B, sb), bias=wide(torch.zeros(N)), out=_share((N, N), bf, big)),
+        lambda: ops.gemm_mxfp4((q, wide(sa)), (B, sb), out=_share((N, N), bf, big)), lambda: ops.gemm_mxfp4((q, sa), (B, wide(sb)), out=_share((N, N), bf, big)),
+        lambda: ops.gemm_mxfp4((wide(q), sa), (B, sb), out=_share((N, N), bf, big)), lambda: ops.gemm_mxfp4((q, sa), (wide(B), sb), out=_share((N, N), bf, big)),
+        lambda: ops.gemm_mxfp4((q8, wide(s8)), (B, sb), out=_share((4, N), bf, big)),
+    ]
+    for n, call in enumerate(calls):
+        with pytest.raises(L.DistError) as e:
+            call()
+        assert "overlaps" in str(e.value), f"call {n}: {e.value}"
+    for call in (lambda: ops.rmsnorm(x, w, res=r, h=x, rstd=rs), lambda: ops.rmsnorm(x, w, res=r, h=r, rstd=rs), lambda: ops.rmsnorm(x, w, res=x, h=x), lambda: ops.rmsnorm_bwd(h, rs, d, w, dres=r, dh=h, dw=dw),
+                 lambda: ops.rmsnorm_bwd(h, rs, d, w, dres=r, dh=d, dw=dw), lambda: ops.rmsnorm_bwd(h, rs, d, w, dres=r, dh=r, dw=dw), lambda: ops.rmsnorm_bwd(h, rs, h, w, dh=h),
+                 lambda: ops.gemm_mxfp4((q, sa), (B, sb), res=x.new_zeros(N, N, dtype=bf), out=x.new_zeros(N, N, dtype=bf)), lambda: ops.gemm_mxfp4((B, sb), (B, sb))):
+        with pytest.raises(L.DistError, match="GPU"):
+            call()
