@@ -391,7 +391,7 @@ __global__ __launch_bounds__(NT_) void gemm_mx_join_kernel(const dist_gemm_mx_ar
 template <bool A8, bool RS, typename TO, int WM, int WN, int MT, int NT, int S, int OCC> int launch_tile(const dist_gemm_mx_args& p, int slice, hipStream_t s) {
     using T = Tile<A8, TO, WM, WN, MT, NT, S>;
     const long ntm = (p.M + T::BM - 1) / T::BM, ntn = (p.N + T::BN - 1) / T::BN, parts = (p.K + slice - 1) / slice;
-    if (ntm * ntn >= 1 << 30 || parts > 65535) return DIST_ERR_ARG;
+    if (mx::too_many(ntm * ntn, 64 * T::W) || parts > 65535) return DIST_ERR_ARG;
     const auto k = gemm_mx_tile_kernel<A8, RS, TO, WM, WN, MT, NT, S, OCC>;
     static DistSmemOnce st;
     RUN_(dist_max_smem(st, reinterpret_cast<const void*>(k), T::LDS));
@@ -426,7 +426,9 @@ Plan plan(int64_t M, int N, int K) {
 }
 
 template <bool A8, typename TO, int MT, int NT, int W> int launch_few(const dist_gemm_mx_args& p, hipStream_t s) {
-    hipLaunchKernelGGL((gemm_mx_few_kernel<A8, TO, MT, NT, W>), dim3((unsigned)((p.N + 16 * NT - 1) / (16 * NT))), dim3(64 * W), 0, s, p);
+    const int64_t blocks = ((int64_t)p.N + 16 * NT - 1) / (16 * NT);
+    if (mx::too_many(blocks, 64 * W)) return DIST_ERR_ARG;
+    hipLaunchKernelGGL((gemm_mx_few_kernel<A8, TO, MT, NT, W>), dim3((unsigned)blocks), dim3(64 * W), 0, s, p);
     HIP_CHECK_RET(hipGetLastError());
     return DIST_OK;
 }
@@ -458,7 +460,7 @@ template <bool A8, typename TO> int launch(const dist_gemm_mx_args& p, hipStream
 }  // namespace
 
 extern "C" int64_t dist_op_gemm_mxfp4_scratch(int64_t M, int N, int K, int a_fmt) {
-    if (M < 0 || N <= 0 || K <= 0 || K % 32 || (a_fmt != DIST_MX_A_MXFP4 && a_fmt != DIST_MX_A_E4M3)) return -1;
+    if (M < 0 || N <= 0 || N > 1 << 30 || K <= 0 || K % 32 || (a_fmt != DIST_MX_A_MXFP4 && a_fmt != DIST_MX_A_E4M3)) return -1;
     const Plan w = plan(M, N, K);
     const int64_t parts = (K + w.slice - 1) / w.slice;
     return parts > 1 ? parts * M * N : 0;
@@ -469,7 +471,7 @@ extern "C" int dist_op_gemm_mxfp4(const dist_gemm_mx_args* a, void* stream) {
     const dist_gemm_mx_args p = *a;
     if (p.a_fmt != DIST_MX_A_MXFP4 && p.a_fmt != DIST_MX_A_E4M3) return DIST_ERR_ARG;
     if ((p.dtype != DIST_BF16 && p.dtype != DIST_F32) || (p.a_fmt == DIST_MX_A_E4M3 && p.dtype != DIST_BF16)) return DIST_ERR_ARG;
-    if (p.M < 0 || p.N <= 0 || p.K <= 0 || p.K % 32 || p.K > LIMIT) return DIST_ERR_ARG;
+    if (p.M < 0 || p.N <= 0 || p.N > 1 << 30 || p.K <= 0 || p.K % 32 || p.K > LIMIT) return DIST_ERR_ARG;
     if (p.M == 0) return DIST_OK;
     const uintptr_t es = p.dtype == DIST_BF16 ? 2 : 4;
     if (!p.A || !p.a_scale || !p.B || !p.b_scale || !p.C || p.ldc < p.N || (p.res && p.ldres < p.N)) return DIST_ERR_ARG;

@@ -21,6 +21,8 @@ DEV int scale_byte(unsigned amax_bits) {
     return e == 255 ? 255 : max(e - 2, 0);
 }
 DEV float scale_value(int byte) { return __uint_as_float(byte == 0 ? 0x00400000u : (unsigned)byte << 23); }   // byte 255: NaN or infinity bits, never used as a divisor
+// a launch takes fewer than 2^32 work items along an axis: these entry points refuse what needs more (DIST_ERR_ARG), before they launch anything
+inline bool too_many(int64_t blocks, int threads) { return blocks > (int64_t)0xffffffffll / threads; }
 // position of block b (of the whole row) inside the scales of `rows` rows
 DEV long scale_at(long row, long rows, int b) { return ((long)(b >> 3) * rows + row) * 8 + 2 * (b & 3) + ((b >> 2) & 1); }
 

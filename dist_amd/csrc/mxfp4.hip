@@ -108,7 +108,7 @@ extern "C" int dist_op_quant_mxfp4(const void* x, int dtype, int64_t rows, int64
     const int64_t Kp = (K + 31) / 32 * 32, chunks = (K + mx::CHUNK - 1) / mx::CHUNK;
     if (!transpose) {
         const int64_t blocks = (rows * chunks + NT / 32 - 1) / (NT / 32);
-        if (blocks > 0x7fffffff) return DIST_ERR_ARG;
+        if (mx::too_many(blocks, NT)) return DIST_ERR_ARG;
         const bool al = cols % 8 == 0 && ld % 8 == 0 && (uintptr_t)x % 16 == 0;
 #define DIST_QR(T, AL) hipLaunchKernelGGL((quant_rows_kernel<T, AL>), dim3((unsigned)blocks), dim3(NT), 0, s, static_cast<const T*>(x), (long)rows, (long)K, (long)ld, (int)Kp, (int)chunks, q, sc)
         if (dtype == DIST_BF16) { if (al) DIST_QR(bf16_t, true); else DIST_QR(bf16_t, false); }
@@ -117,7 +117,7 @@ extern "C" int dist_op_quant_mxfp4(const void* x, int dtype, int64_t rows, int64
     } else {
         const bool two = dtype == DIST_BF16 && cols % 2 == 0 && ld % 2 == 0 && (uintptr_t)x % 4 == 0;        // two bf16 columns a lane
         const int64_t ctiles = two ? (cols + 127) / 128 : (cols + 63) / 64, blocks = ctiles * chunks;
-        if (blocks > 0x7fffffff) return DIST_ERR_ARG;
+        if (mx::too_many(blocks, 512)) return DIST_ERR_ARG;
 #define DIST_QC(T, VC) hipLaunchKernelGGL((quant_cols_kernel<T, VC>), dim3((unsigned)blocks), dim3(512), 0, s, static_cast<const T*>(x), (long)rows, (int)cols, (long)ld, (long)Kp, (int)ctiles, q, sc)
         if (two) DIST_QC(bf16_t, 2); else if (dtype == DIST_BF16) DIST_QC(bf16_t, 1); else DIST_QC(float, 1);
 #undef DIST_QC
@@ -131,7 +131,7 @@ extern "C" int dist_op_dequant_mxfp4(const void* codes, const void* scales, int6
     if (rows == 0) return DIST_OK;
     if (!codes || !scales || !y || (uintptr_t)codes % 16 || (uintptr_t)y % 16) return DIST_ERR_ARG;
     const int64_t blocks = (rows * (K / 8) + NT - 1) / NT;
-    if (blocks > 0x7fffffff) return DIST_ERR_ARG;
+    if (mx::too_many(blocks, NT)) return DIST_ERR_ARG;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const unsigned char *q = static_cast<const unsigned char*>(codes), *sc = static_cast<const unsigned char*>(scales);
     if (dtype == DIST_BF16) hipLaunchKernelGGL(dequant_kernel<bf16_t>, dim3((unsigned)blocks), dim3(NT), 0, s, q, sc, (long)rows, (int)K, static_cast<bf16_t*>(y));

@@ -288,21 +288,23 @@ __global__ __launch_bounds__(LPR > NT ? LPR : NT, 2) void rms_bwd_kernel(const d
     }
 }
 
-// long rows: dh by a block per row; dw by columns, one partial row per slice of rows
+// long rows, and rows of less than a group: dh by a block per row (of many rows: the workgroups stride over them); dw by columns, one partial row per slice of rows
+constexpr int64_t LONG_BLOCKS = 1 << 20;
 template <typename T, typename TD>
 __global__ __launch_bounds__(NT) void rms_bwd_long_kernel(const dist_rms_bwd_args p) {
     __shared__ float red[4];
-    const long row = blockIdx.x;
     const int C = p.C;
-    const T* H = static_cast<const T*>(p.h) + row * p.ldh;
-    const TD* D = static_cast<const TD*>(p.dy) + row * p.lddy;
-    const T* A = p.dres ? static_cast<const T*>(p.dres) + row * p.lddres : nullptr;
-    T* O = static_cast<T*>(p.dh) + row * p.lddh;
-    const float rstd = p.rstd[row];
-    float s = 0.f;
-    for (long c = threadIdx.x; c < C; c += NT) s += to_f(D[c]) * p.w[c] * (to_f(H[c]) * rstd);
-    const float m = row_sum<NT>(s, red) / (float)C;
-    for (long c = threadIdx.x; c < C; c += NT) O[c] = from_f<T>(rstd * (to_f(D[c]) * p.w[c] - to_f(H[c]) * rstd * m) + (A ? to_f(A[c]) : 0.f));
+    for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T* H = static_cast<const T*>(p.h) + row * p.ldh;
+        const TD* D = static_cast<const TD*>(p.dy) + row * p.lddy;
+        const T* A = p.dres ? static_cast<const T*>(p.dres) + row * p.lddres : nullptr;
+        T* O = static_cast<T*>(p.dh) + row * p.lddh;
+        const float rstd = p.rstd[row];
+        float s = 0.f;
+        for (long c = threadIdx.x; c < C; c += NT) s += to_f(D[c]) * p.w[c] * (to_f(H[c]) * rstd);
+        const float m = row_sum<NT>(s, red) / (float)C;
+        for (long c = threadIdx.x; c < C; c += NT) O[c] = from_f<T>(rstd * (to_f(D[c]) * p.w[c] - to_f(H[c]) * rstd * m) + (A ? to_f(A[c]) : 0.f));
+    }
 }
 template <typename T, typename TD>
 __global__ __launch_bounds__(NT) void rms_dw_cols_kernel(const dist_rms_bwd_args p, const int slices, const int ctiles) {
@@ -350,7 +352,7 @@ inline bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 template <typename T, bool AL, int FMT> int fwd(const dist_rms_args& p, hipStream_t s) {
     const int64_t Cr = FMT == DIST_RMS_MXFP4 ? ((int64_t)p.C + 255) / 256 * 256 : p.C;       // (the scale bytes of a whole chunk are written)
     const int64_t rows = p.rows;
-#define DIST_RMS(LPR, IT) do { const int64_t b = (rows + NT / LPR - 1) / (NT / LPR); if (b > 0x7fffffff) return DIST_ERR_ARG; \
+#define DIST_RMS(LPR, IT) do { const int64_t b = (rows + NT / LPR - 1) / (NT / LPR); if (mx::too_many(b, NT)) return DIST_ERR_ARG; \
         hipLaunchKernelGGL((rms_fwd_kernel<T, AL, LPR, IT, FMT>), dim3((unsigned)b), dim3(NT), 0, s, p); } while (0)
     if (Cr <= 384) DIST_RMS(16, 3);
     else if (Cr <= 768) DIST_RMS(32, 3);
@@ -360,7 +362,7 @@ template <typename T, bool AL, int FMT> int fwd(const dist_rms_args& p, hipStrea
     else if (Cr <= 8192) DIST_RMS(256, 4);
     else if (Cr <= FWD_MAX) DIST_RMS(256, 8);
     else {
-        if (rows > 0x7fffffff) return DIST_ERR_ARG;
+        if (mx::too_many(rows, NT)) return DIST_ERR_ARG;
         hipLaunchKernelGGL((rms_fwd_long_kernel<T, FMT>), dim3((unsigned)rows), dim3(NT), 0, s, p);
     }
 #undef DIST_RMS
@@ -377,11 +379,13 @@ template <typename T, typename TD, bool AL> int bwd(const dist_rms_bwd_args& p, 
     const int G = (int)bwd_partials(p.rows, p.C);
     const int lanes = bwd_lanes(p.C);
 #define DIST_RMS(LPR, IT) hipLaunchKernelGGL((rms_bwd_kernel<T, TD, AL, LPR, IT>), dim3((unsigned)G), dim3(LPR > NT ? LPR : NT), 0, s, p)
+    const int64_t sums = (p.C + 15) / 16;                     // workgroups of the last pass
+    if (mx::too_many(sums, 1024)) return DIST_ERR_ARG;
     if (!lanes) {
-        if (p.rows > 0x7fffffff) return DIST_ERR_ARG;
         const int ctiles = (p.C + NT - 1) / NT;
+        if (mx::too_many((int64_t)G * ctiles, NT)) return DIST_ERR_ARG;
         hipLaunchKernelGGL((rms_dw_cols_kernel<T, TD>), dim3((unsigned)(G * ctiles)), dim3(NT), 0, s, p, G, ctiles);       // (before dh, which may take h's or dy's place)
-        if (p.dh && p.rows) hipLaunchKernelGGL((rms_bwd_long_kernel<T, TD>), dim3((unsigned)p.rows), dim3(NT), 0, s, p);
+        if (p.dh && p.rows) hipLaunchKernelGGL((rms_bwd_long_kernel<T, TD>), dim3((unsigned)min(p.rows, LONG_BLOCKS)), dim3(NT), 0, s, p);
     } else if (lanes == 16) DIST_RMS(16, 3);
     else if (lanes == 32) DIST_RMS(32, 3);
     else if (lanes == 64) DIST_RMS(64, 2);
@@ -390,7 +394,7 @@ template <typename T, typename TD, bool AL> int bwd(const dist_rms_bwd_args& p, 
 #undef DIST_RMS
     HIP_CHECK_RET(hipGetLastError());
     if (lanes && G == 1) return DIST_OK;
-    hipLaunchKernelGGL(rms_dw_kernel, dim3((unsigned)((p.C + 15) / 16)), dim3(1024), 0, s, p.scratch, G, p.C, p.dw, p.accumulate);
+    hipLaunchKernelGGL(rms_dw_kernel, dim3((unsigned)sums), dim3(1024), 0, s, p.scratch, G, p.C, p.dw, p.accumulate);
     HIP_CHECK_RET(hipGetLastError());
     return DIST_OK;
 }

@@ -140,7 +140,9 @@ int dist_op_fp8_rowsum(const void* q, const float* scale, int64_t rows, int K, i
  *   DIST_RMS_E4M3:  y [rows][ldy] bytes, scale fp32 [rows]: what dist_op_quant_rows_fp8 makes of the unrounded y (a row whose largest |y| is below 2^-100 is scaled
  *                   as if it were 2^-100); operands of dist_op_gemm_nt (DIST_EPI_FP8) and dist_op_gemm_mxfp4
  *   DIST_RMS_MXFP4: y codes, scale bytes: what dist_op_quant_mxfp4 makes of the unrounded y; y 16-byte aligned, ldy unused
- * Any C and any alignment of whole elements; C % 8 == 0 with 16-byte aligned rows is the fast form.  rows = 0 is nothing to do. */
+ * Any C up to 2^30 and any alignment of whole elements; C % 8 == 0 with 16-byte aligned rows is the fast form.  rows = 0 is nothing to do.
+ * (This layer's calls whose launch would need 2^32 work items are refused with DIST_ERR_ARG: 2^28 rows of up to 384 elements here, fewer of longer ones; 2^35 elements or
+ * 2^27 rows to quantise or to read back; a weight of 2^27 rows.) */
 enum { DIST_RMS_SAME = 0, DIST_RMS_E4M3 = 1, DIST_RMS_MXFP4 = 2 };
 typedef struct dist_rms_args {
     const void* x; const void* res; void* h; const float* w; void* y; void* scale; float* rstd;
@@ -150,7 +152,7 @@ typedef struct dist_rms_args {
 int dist_op_rmsnorm(const dist_rms_args* a, void* stream);
 /* Backward from the stored h and rstd: g = dy * w, n = h * rstd, dh = rstd * (g - n * mean_c(g n)) + dres (dres optional: the gradient that reaches h past the norm),
  * dw[c] (+)= sum_rows dy n in a fixed order (accumulate: added to what dw holds).  h, dres, dh in `dtype`, dy in `dy_dtype`, dw fp32 [C].  dh is optional and may be dres or,
- * where the types agree, h or dy.  scratch: fp32, >= dist_op_rmsnorm_bwd_scratch(rows, C) elements.  rows = 0: dw = 0 (or unchanged). */
+ * where the types agree, h or dy.  C <= 2^26 - 256.  scratch: fp32, >= dist_op_rmsnorm_bwd_scratch(rows, C) elements.  rows = 0: dw = 0 (or unchanged). */
 typedef struct dist_rms_bwd_args {
     const void* h; const float* rstd; const void* dy; const float* w; const void* dres; void* dh; float* dw; float* scratch;
     int64_t scratch_elems, rows, ldh, lddy, lddres, lddh;
@@ -172,7 +174,7 @@ int dist_op_dequant_mxfp4(const void* codes, const void* scales, int64_t rows, i
  *   DIST_MX_A_MXFP4: A codes [M][K / 2], a_scale its scale bytes; C and res in `dtype` (bf16 / fp32)
  *   DIST_MX_A_E4M3:  A e4m3 bytes [M][lda] (lda % 16 == 0), a_scale fp32 [M]; C and res in bf16 only: the matrix instruction aligns every eight products of an e4m3
  *                    operand to the largest of them and keeps 13 bits below it, far inside a bf16 result and outside an fp32 one
- * fp32 sums; bias fp32 [N] and res [M][ldres] optional; res may be C.  Codes 16-byte, scale bytes 8-byte aligned.  M = 0 is nothing to do.
+ * K and lda up to 2^22.  fp32 sums; bias fp32 [N] and res [M][ldres] optional; res may be C.  Codes 16-byte, scale bytes 8-byte aligned.  M = 0 is nothing to do.
  * Gradients are the same call on other operands: dA = Q(dC) Q(B^T)^T, dB = Q(dC^T) Q(A^T)^T (transpose above).
  * scratch: fp32, >= dist_op_gemm_mxfp4_scratch(M, N, K, a_fmt) elements (0 for most sizes). */
 enum { DIST_MX_A_MXFP4 = 0, DIST_MX_A_E4M3 = 1 };

@@ -43,3 +43,21 @@ def test_norm_beside_its_input(C, gpu_lib):
     same_bits(a, x)
     for u, v in zip(got, want):
         same_bits(u, v)
+
+
+@pytest.mark.parametrize("rows,C", [((1 << 20) + 5, 2), ((1 << 24) + 3, 3), ((1 << 20) + 1, 7)])
+def test_norm_gradient_of_more_short_rows_than_workgroups(rows, C, gpu_lib):
+    h = torch.randn(rows, C, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(BF)
+    d = torch.randn(rows, C, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").to(BF)
+    w = torch.rand(C, generator=gen(3)).cuda()
+    rstd = 1 / torch.sqrt(h.float().square().mean(1) + 1e-6)
+    dh, dw = ops.rmsnorm_bwd(h, rstd, d, w)
+    n, g = h.double() * rstd.double()[:, None], d.double() * w.double()
+    want = rstd.double()[:, None] * (g - n * (g * n).mean(1, keepdim=True))
+    # as test_norm_gradient's: every addition and product around the sum of C terms
+    inner = rstd.double()[:, None] * (4 * g.abs() + n.abs() * ((C + 8 + 4) * (g * n).abs().mean(1, keepdim=True) + 6 * (g * n).mean(1, keepdim=True).abs()))
+    assert bool(((dh.double() - want).abs() <= half(BF) * want.abs() + 1.01 * U * inner).all())
+    # a slice's chain of rows, 64 slices, and the products
+    assert bool(((dw.double() - (d.double() * n).sum(0)).abs() <= (rows // 64 + 64 + 4) * U * (d.double() * n).abs().sum(0)).all())
+    c = h.clone()
+    same_bits(ops.rmsnorm_bwd(c, rstd, d, w, dh=c)[0], dh)
