@@ -407,19 +407,23 @@ enum { FEW = 0, SMALL = 1, SQUARE = 2, BIG = 3 };
 struct Plan { int kind, slice; };
 constexpr int LIMIT = 1 << 22;                               // bytes of a row (the 256 rows of a tile lie within 32-bit offsets)
 
-// Which kernel (times in us, inputs out of the caches, bias; kernels of this file beside each other):
-//   FEW     M <= 64: the tiles' ring has a long way to the first result.  N = K = 4096: 64 rows 9.1 against 10.9 in 64 x 64 tiles, 16 rows 4.8
-//   SMALL   64 x 64, where 128 x 128 would leave CUs without work (under 200 tiles): 788 x 2304 x 768 4.9 against 5.9; 2048 x 2048 x 1024 (256 tiles) 8.4 against 6.4 the other way.
+// Which kernel (times in us, inputs out of the caches, bf16 out, bias; kernels of this file beside each other, the middle of seven graphs in turn):
+//   FEW     M <= 64.  N = K = 4096: 16 rows 5.2 against 8.7 in 64 x 64 tiles, 48 rows 8.2 against 8.7, 64 rows 9.2 against 8.9.  Its time grows with the rows and with N, that of
+//           the tiles hardly: with wide weights they would be the faster from 17 rows on (24 x 16384 x 4096 15.5 against 9.4, 64 x 8192 x 8192 26 against 14.6)
+//   SMALL   64 x 64, where 128 x 128 would leave CUs without work (under 200 tiles): 788 x 2304 x 768 5.0 against 5.6; 2048 x 2048 x 1024 (256 tiles) 9.3 against 6.9 the other way.
+//           2304 x 768 x 12608 (108 tiles) 33.5 against 43.4.
 //           The long axis is cut where even these do not fill the 256 CUs, in slices of at least 2048 (shorter ones cost more in the joining pass than they gain:
-//           200 x 520 x 2048 7.1 whole, 7.7 in two)
+//           200 x 520 x 2048 6.0 whole, 6.9 in two).  768 x 768 x 12608 (144 tiles) is 20.8 whole, 23.4 in two
 //   SQUARE  128 x 128, two workgroups a CU (e4m3: three)
-//   BIG     256 x 256, one a CU: four times the work of SQUARE, so it wins where its rounds over the 256 CUs are full, by 6 % and more.  4-bit rows: 4096^3 39 against 44,
-//           6400 x 2304 x 768 (225 tiles) 12.6 against 13.4, but 16448 x 1024 x 4096 (260 tiles) 68 against 56;  e4m3 rows: 8192^3 380 (2.9 PF) against 414,
-//           50432 x 2304 x 768 101 against 104, 16384 x 1024 x 4096 56 against 63, but 12608 x 2304 x 768 (450 tiles) 29 against 27
-Plan plan(int64_t M, int N, int K) {
+//   BIG     256 x 256, one a CU: four times the work of SQUARE, so it wins where its rounds over the 256 CUs are full.  4-bit rows: 4096^3 38.5 against 43, 8192^3 264 against 291,
+//           32768 x 1024 x 4096 78 against 88, 6400 x 2304 x 768 (225 tiles) 12.9 against 14.1, but 16448 x 1024 x 4096 (260 tiles) 63 against 51.
+//           e4m3 rows: only in a single round, or with a long axis beside which the outputs are short - nothing else runs on the CU while its one workgroup stores, and SQUARE has three:
+//           4096^3 55 against 58, 16384 x 1024 x 4096 54 against 57.5, 6400 x 2304 x 768 16.5 against 17.9, 32768 x 1024 x 4096 118 against 131, 8192^3 416 against 414, but several rounds
+//           of short axes 50432 x 2304 x 768 108 against 98, 25600 x 2304 x 768 61 against 54, 16384 x 2048 x 2048 63 against 59
+Plan plan(int64_t M, int N, int K, bool a8) {
     const int64_t t64 = (M + 63) / 64 * ((N + 63) / 64), t128 = (M + 127) / 128 * ((N + 127) / 128), t256 = (M + 255) / 256 * ((N + 255) / 256);
     if (M <= 64) return Plan{FEW, K};
-    if (t128 >= 200) return Plan{15 * ((t256 + 255) / 256) <= 4 * ((t128 + 255) / 256) ? BIG : SQUARE, K};
+    if (t128 >= 200) return Plan{15 * ((t256 + 255) / 256) <= 4 * ((t128 + 255) / 256) && (!a8 || t256 <= 256 || K >= 4096) ? BIG : SQUARE, K};
     int parts = 1;
     while (t64 * parts < 256 && K / (2 * parts) >= 2048) parts *= 2;
     return Plan{SMALL, parts == 1 ? K : (K / parts + 255) / 256 * 256};
@@ -434,7 +438,7 @@ template <bool A8, typename TO, int MT, int NT, int W> int launch_few(const dist
 }
 
 template <bool A8, typename TO> int launch(const dist_gemm_mx_args& p, hipStream_t s) {
-    Plan w = plan(p.M, p.N, p.K);
+    const Plan w = plan(p.M, p.N, p.K, A8);
     if (w.kind == FEW) {
         if (p.M <= 16) return launch_few<A8, TO, 1, 1, 8>(p, s);
         if (p.M <= 32) return launch_few<A8, TO, 2, 1, 8>(p, s);
@@ -461,7 +465,7 @@ template <bool A8, typename TO> int launch(const dist_gemm_mx_args& p, hipStream
 
 extern "C" int64_t dist_op_gemm_mxfp4_scratch(int64_t M, int N, int K, int a_fmt) {
     if (M < 0 || N <= 0 || N > 1 << 30 || K <= 0 || K % 32 || (a_fmt != DIST_MX_A_MXFP4 && a_fmt != DIST_MX_A_E4M3)) return -1;
-    const Plan w = plan(M, N, K);
+    const Plan w = plan(M, N, K, a_fmt == DIST_MX_A_E4M3);
     const int64_t parts = (K + w.slice - 1) / w.slice;
     return parts > 1 ? parts * M * N : 0;
 }
