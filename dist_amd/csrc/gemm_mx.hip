@@ -45,7 +45,6 @@ __global__ __launch_bounds__(64 * W) void gemm_mx_few_kernel(const dist_gemm_mx_
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const v4i_t zero = {0, 0, 0, 0};
-#pragma unroll 2
     for (int k = wave * 128; k < p.K; k += W * 128) {
         const long chunk = k >> 8;
         const int at = 2 * g + ((k >> 7) & 1);
@@ -101,9 +100,10 @@ __global__ __launch_bounds__(64 * W) void gemm_mx_few_kernel(const dist_gemm_mx_
 // every wave and stage t - 1 is read by nobody, so its place receives stage t + S - 1.  Scale bytes follow per 256 elements into a ring of their own, with the stage that needs
 // them first.  A 16-byte chunk c of row r lies at chunk c ^ f(r), applied where the DMA reads (its LDS side is lane-linear).  Descriptors end behind the last row, and chunks
 // behind K are sent past the end: all of these read as zeros.
-// Measured (50432 x 2304 x 768, 4-bit operands, bf16 out): 83 us = 2.15 PF (stages of 128 elements: 95); of it 43 us are the outputs' stores (5.4 TB/s), which with three
-// stages a tile add to the loop more than they hide behind it.  4096^3: 38 us = 3.6 PF.  e4m3 rows: 8192^3 379 us = 2.9 PF; 24576 x 1024 x 4096 98 us = 2.1 PF, the matrix
-// units busy 54 % of the clocks (1.87 GHz) and the LDS reads 23 %: the three workgroups of a CU wait at their barriers at much the same time.
+// Measured, in graphs: 50432 x 2304 x 768, 4-bit operands, bf16 out, 79 us = 2.25 PF in 256 x 256 tiles and 82 in 128 x 128 (stages of 128 elements: 95); of it 43 us are the outputs' stores
+// (5.4 TB/s), which with three stages a tile add to the loop more than they hide behind it.  4096^3: 38.5 us = 3.6 PF; 8192^3 264 us = 4.2 PF.  e4m3 rows: 8192^3 416 us = 2.65 PF;
+// 24576 x 1024 x 4096 103 us = 2.0 PF in 128 x 128 tiles; of its clocks (87 us at 2.08 GHz one at a time) the matrix units are busy 54 % and the LDS 24 %: the three workgroups of a CU
+// wait at their barriers at much the same time.  A width or pitch that 16-byte pieces do not divide takes the element-wise epilogue, many times slower: 50432 x 2299 x 768 340 us.
 // Built and not faster: workgroups that stay and prefetch across tiles (in both depths of stages); in stages of 128 fragments read half a stage ahead, three or four stages in
 // the ring, all reads in front of the matrix instructions, raised priority around them (all within 5 %).
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -117,7 +117,7 @@ template <typename TO> DEV constexpr int frag_col(int j) { return sizeof(TO) == 
 template <typename TO> DEV int lane_col(int i) { return sizeof(TO) == 2 ? (i >> 2) * 8 + (i & 3) : i; }
 
 // (8 lanes read 128 bytes at a time: their 8 rows - consecutive ones of A, 0 ... 3 and 8 ... 11 of a 16-bit B - must fall on different 16-byte places.  ds_read_b128 then
-// moves 234 bytes a clock and CU; patterns that are free of conflicts over 16 lanes only reach 127.)
+// moves about 240 bytes a clock and CU; patterns that are free of conflicts over 16 lanes only reach 126.)
 DEV int a_swz(int r) { return (r >> 1) & 7; }
 template <typename TO> DEV int b_swz(int r) { return sizeof(TO) == 2 ? ((r >> 1) & 1) | ((r >> 2) & 2) : (r >> 1) & 3; }
 

@@ -336,7 +336,9 @@ __global__ __launch_bounds__(1024) void rms_dw_kernel(const float* __restrict__ 
 }
 
 constexpr int FWD_MAX = 16384, BWD_MAX = 8192;                // widths whose rows stay in registers
-constexpr int PARTIALS = 512;                                  // workgroups of the backward kernel, two a CU (50432 x 768: 384 67 us, 512 62, 640 77, 1024 66)
+// Workgroups of the backward kernel: two a CU of 256 threads each (50432 x 768: 384 67 us, 512 62, 640 77, 1024 66).  Of the 512 threads that rows over 4096 take a CU holds one
+// (150 registers and more a lane), so that these run in two rounds of it (1831 x 8192 bf16 38.5 us for 92 MB; not tried with 256).
+constexpr int PARTIALS = 512;
 
 // lanes per row of the backward kernel (0: a long row, or one of less than a group).  At most three groups of eight a lane, else a CU holds one workgroup only (15 M elements in bf16: 2048 columns by 64 lanes
 // of four groups 29.6 us, by 256 of one 27.6; 8192 by 256 of four 40.3, by 512 of two 38.6)
