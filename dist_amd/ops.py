@@ -623,11 +623,14 @@ def _meet(a, b):
 def _apart(out, what, *inputs, may_be=True):
     """an output that the caller brings may be one of these operands itself (same address, type, shape and pitch; not with may_be=False) but must not overlap them otherwise"""
     mine = _runs(out)
-    end = mine[0] + (mine[3] - 1) * mine[2] + mine[1]
+    first, end = mine[0], mine[0] + (mine[3] - 1) * mine[2] + mine[1]
     for t in inputs:
-        if t is None or t.data_ptr() >= end:
+        if t is None:
             continue
-        if may_be and mine[0] == t.data_ptr() and out.dtype == t.dtype and out.shape == t.shape and (out.shape[0] == 1 or out.stride(0) == t.stride(0)):
+        at = t.data_ptr()
+        if at >= end or (at + t.nbytes <= first and t.is_contiguous()):
+            continue
+        if may_be and at == first and out.dtype == t.dtype and out.shape == t.shape and (out.shape[0] == 1 or out.stride(0) == t.stride(0)):
             continue
         other = _runs(t)
         if mine[1] and other[1] and _meet(mine, other):
@@ -793,8 +796,9 @@ def gemm_mxfp4(A, B, *, bias=None, res=None, out=None, out_dtype=torch.bfloat16)
     ldres = _matrix(res, (M, N), "res", out_dtype if out is None else out.dtype) if res is not None else 0
     if out is not None:
         ldc = _matrix(out, (M, N), "out", out.dtype)
-        _apart(out, "out", res)
-        _apart(out, "out", q, sc, *B, bias, may_be=False)
+        if res is not None:
+            _apart(out, "out", res)
+        _apart(out, "out", q, sc, B[0], B[1], bias, may_be=False)
     dev = _device(q, sc, B[0], B[1], bias, res, out)
     if out is None:
         out, ldc = torch.empty(M, N, dtype=out_dtype, device=q.device), N
