@@ -671,7 +671,7 @@ __global__ __launch_bounds__(Shape<NW>::NT, Shape<NW>::MINB) void gemm_fast_kern
 //   RAW: a half-tile is read in L(g) only if every wave waited for its own pieces of it (counted vmcnt) at the end of
 //        L(g-1) or earlier - that wait is followed by a barrier both groups pass before any read of L(g);
 //   WAR: every wave retires the reads of L(g) (lgkmcnt(0)) at the END of M(g), in front of the barrier that closes it, so
-//        a half-tile last read in L(g) may be re-staged in L(g+2) by either group.
+//        a half-tile last read in L(g) may be re-staged in L(g+2) by either group.  The prologue's reads count as an L of their own: a barrier closes them.
 // Per-wave LDS-DMA issue order is A-h0, B-h0, B-h1, A-h1 of a tile, two pieces each, tile t+2 during tile t: `vmcnt(10)`
 // at the end of every load section leaves five half-tiles in flight and retires exactly the one the NEXT load section reads.
 //
@@ -923,6 +923,7 @@ __global__ __launch_bounds__(512, 1) void gemm_fast8p_kernel(const dist_gemm_arg
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     regs_ready(fa[0]); regs_ready(sb_[0]);
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();                         // group 0's first load section stages A-h0 of tile 2 over the A-h0 that a slower wave of it may still be reading here
     if (wr == 1) __builtin_amdgcn_s_barrier();            // group 1 runs one barrier interval behind group 0
     using I0 = std::integral_constant<int, 0>; using I1 = std::integral_constant<int, 1>;
     int kt = 0;

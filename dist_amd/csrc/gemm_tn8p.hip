@@ -220,6 +220,7 @@ __global__ __launch_bounds__(512, 1) void gemm_tn8r_kernel(const dist_gemm_tn_ar
     asm volatile("" : "+v"(fa[0][0]), "+v"(fa[0][1]), "+v"(fa[0][2]), "+v"(sb_[0][0]), "+v"(sb_[0][1]));
     colsum_q(0);
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();                              // group 0's first phase stages over slot 0, which a slower wave may still be reading here
     if (wr == 1) __builtin_amdgcn_s_barrier();
 #pragma unroll 1
     for (int body = 0; body < nbody; ++body) {

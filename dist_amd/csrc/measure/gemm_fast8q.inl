@@ -247,6 +247,7 @@ __global__ __launch_bounds__(512, 1) void gemm_fast8q_kernel(const dist_gemm_arg
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     regs_ready(fa[0]); regs_ready(sb_[0]);
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();                         // (group 0's first load section stages over what a slower wave may still be reading)
     if (wr == 1) __builtin_amdgcn_s_barrier();
     using I0 = std::integral_constant<int, 0>; using I1 = std::integral_constant<int, 1>;
 #pragma unroll 1
